@@ -26,6 +26,7 @@ TENSOR_A, TENSOR_B, TENSOR_C = 1, 2, 3
 EXPORTS = [
     "b200_gemm_default_params", "b200_gemm_default_params_plain", "b200_gemm_default_params_for_call", "b200_gemm_validate", "b200_gemm_smem_bytes", "b200_gemm_workspace_bytes", "b200_gemm_schedule",
     "b200_gemm_f16", "b200_gemm_bf16", "b200_gemm_f16_out_f16", "b200_gemm_splitk_noalloc", "b200_gemm_push", "b200_push_reduce",
+    "b200_gemm_lora", "b200_gemm_lora_workspace_bytes", "b200_moe", "b200_moe_workspace_bytes",
     "b200_peer_alloc", "b200_peer_free", "b200_peer_export", "b200_peer_import", "b200_peer_release", "b200_session_create", "b200_session_destroy", "b200_session_gemm_host", "b200_session_buffers", "b200_session_gemm_host_sharded",
     "b200_device_status", "b200_set_wait_budget_ns", "b200_set_profile_buffer", "b200_profile_slots", "b200_status_string", "b200_last_cuda_error", "b200_num_sms",
     "b200_fill_u16_device", "b200_fill_f32_device", "b200_fill_u16_host", "b200_fill_f32_host",
@@ -93,6 +94,14 @@ def lib():
         L.b200_session_buffers.argtypes = [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]
         L.b200_session_gemm_host_sharded.argtypes = [vp, C.c_int, vp, vp, vp, vp, f32, f32, i64, i64, i64, C.c_int, C.c_int,
                                                      C.POINTER(vp), C.POINTER(vp), C.c_int, PP]
+        L.b200_gemm_lora_workspace_bytes.argtypes = [i64, i64, i64, i64, C.c_int]
+        L.b200_gemm_lora_workspace_bytes.restype = i64
+        L.b200_gemm_lora.argtypes = [C.c_int, vp, vp, vp, i64, i64, i64, vp, vp, vp, vp, i64, C.c_int, vp, sz, vp]
+        L.b200_gemm_lora.restype = C.c_int
+        L.b200_moe_workspace_bytes.argtypes = [i64, i64, i64, i64, C.c_int]
+        L.b200_moe_workspace_bytes.restype = i64
+        L.b200_moe.argtypes = [C.c_int, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, C.c_int, C.c_int, vp, sz, vp]
+        L.b200_moe.restype = C.c_int
         L.b200_device_status.argtypes = [vp, C.POINTER(C.c_int * 4)]
         L.b200_set_wait_budget_ns.argtypes = [u64]
         L.b200_set_wait_budget_ns.restype = None
@@ -246,6 +255,127 @@ def gemm(A, Bt, Cm=None, D=None, alpha=1.0, beta=0.0, params: Params | None = No
     if st != OK:
         raise B200Error(st, "b200_gemm")
     return D
+
+
+def _require(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _check_operands(where: str, device, *named) -> None:
+    """named: (name, tensor, dtype, shape); a tensor of None passes."""
+    for name, t, dtype, shape in named:
+        if t is not None and not (t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous()):
+            raise ValueError(f"{where}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
+                             f"not {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
+
+
+class _On:
+    """Makes a tensor's device and the stream of the call current, so that what is allocated for the call (outputs, the
+    workspace) belongs to that stream. Does nothing where both are current already, the usual case."""
+
+    def __init__(self, device, stream):
+        import torch
+        now = torch.cuda.current_stream(device)
+        self.stream = now.cuda_stream if stream is None else int(stream)
+        self.guard = None
+        if device.index != torch.cuda.current_device() or self.stream != now.cuda_stream:
+            on = now if self.stream == now.cuda_stream else torch.cuda.ExternalStream(self.stream, device) if self.stream else torch.cuda.default_stream(device)
+            self.guard = torch.cuda.stream(on)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def gemm_lora_workspace_bytes(M, N, K, num_adapters, rank) -> int:
+    """b200_gemm_lora_workspace_bytes; -1 for sizes that the call refuses."""
+    return lib().b200_gemm_lora_workspace_bytes(M, N, K, num_adapters, rank)
+
+
+def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, workspace=None, stream=None):
+    """D[i] = A[i] @ Bt.T + lora_scale[s] * (A[i] @ lora_a[s].T) @ lora_b[s].T with s = row_adapter[i]: a projection shared by all
+    rows with low-rank adapters of many requests beside it (b200_gemm_lora).
+
+    A (m, k), Bt (n, k), lora_a (adapters, rank, k), lora_b (adapters, n, rank) and D (m, n): contiguous torch CUDA tensors of
+    one 16-bit type; row_adapter (m,) int32, an entry outside [0, adapters) = no adapter; lora_scale (adapters,) fp32 or None.
+    D and the workspace are allocated, on the stream of the call, when not given. stream: a cudaStream_t as an int (None =
+    torch's current one); the operands must be ready there. Raises ValueError for tensors that do not fit together and
+    B200Error for what the library refuses."""
+    import torch
+    _require(A.is_cuda and A.dtype in (torch.float16, torch.bfloat16) and A.dim() == 2, "gemm_lora: A must be a 2-d fp16 or bf16 CUDA tensor")
+    _require(Bt.dim() == 2 and lora_a.dim() == 3, "gemm_lora: Bt must have 2 dimensions and lora_a 3")
+    M, K = A.shape
+    N = Bt.shape[0]
+    S, R = lora_a.shape[0], lora_a.shape[1]
+    dev, t = A.device, A.dtype
+    _check_operands("gemm_lora", dev, ("A", A, t, (M, K)), ("Bt", Bt, t, (N, K)), ("lora_a", lora_a, t, (S, R, K)), ("lora_b", lora_b, t, (S, N, R)),
+                    ("row_adapter", row_adapter, torch.int32, (M,)), ("lora_scale", lora_scale, torch.float32, (S,)), ("D", D, t, (M, N)))
+    L = lib()
+    with _On(dev, stream) as sptr:
+        need = L.b200_gemm_lora_workspace_bytes(M, N, K, S, R)
+        if workspace is None and need > 0:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        if D is None:
+            D = torch.empty((M, N), dtype=t, device=dev)
+        st = L.b200_gemm_lora(BF16 if t == torch.bfloat16 else F16, A.data_ptr(), Bt.data_ptr(), D.data_ptr(), M, N, K, lora_a.data_ptr(),
+                              lora_b.data_ptr(), _ptr(lora_scale), row_adapter.data_ptr(), S, R, _ptr(workspace),
+                              workspace.numel() * workspace.element_size() if workspace is not None else 0, sptr)
+    if st != OK:
+        raise B200Error(st, "b200_gemm_lora")
+    return D
+
+
+def moe_workspace_bytes(tokens, hidden, inner, experts, top_k) -> int:
+    """b200_moe_workspace_bytes; -1 for sizes that the call refuses."""
+    return lib().b200_moe_workspace_bytes(tokens, hidden, inner, experts, top_k)
+
+
+def moe(X, logits, W13, W2, top_k, normalise=True, Y=None, ids=None, weights=None, workspace=None, stream=None):
+    """A whole mixture-of-experts layer for a few tokens (b200_moe): returns (Y, ids, weights).
+
+    X (tokens, hidden), W13 (experts, 2 * inner, hidden: the gate's rows, then the others), W2 (experts, hidden, inner) and Y like X:
+    contiguous torch CUDA tensors of one 16-bit type; logits (tokens, experts) fp32, what gemm() returns for the router's
+    product; ids (tokens, top_k) int32 and weights (tokens, top_k) fp32 are the router's choice, in descending order of the
+    logits. Outputs and the workspace are allocated, on the stream of the call, when not given; stream as in gemm_lora.
+    Raises ValueError for tensors that do not fit together and B200Error for what the library refuses."""
+    import torch
+    _require(X.is_cuda and X.dtype in (torch.float16, torch.bfloat16) and X.dim() == 2, "moe: X must be a 2-d fp16 or bf16 CUDA tensor")
+    _require(W2.dim() == 3, "moe: W2 must have 3 dimensions")
+    T, H = X.shape
+    E, I = W2.shape[0], W2.shape[2]
+    dev, t = X.device, X.dtype
+    _check_operands("moe", dev, ("X", X, t, (T, H)), ("logits", logits, torch.float32, (T, E)), ("W13", W13, t, (E, 2 * I, H)), ("W2", W2, t, (E, H, I)),
+                    ("Y", Y, t, (T, H)), ("ids", ids, torch.int32, (T, top_k)), ("weights", weights, torch.float32, (T, top_k)))
+    L = lib()
+    with _On(dev, stream) as sptr:
+        need = L.b200_moe_workspace_bytes(T, H, I, E, top_k)
+        if need < 0:      # refused; the call says why
+            st = L.b200_moe(BF16 if t == torch.bfloat16 else F16, None, None, None, None, None, None, None, T, H, I, E, top_k, int(normalise), None, 0, sptr)
+            raise B200Error(st, "b200_moe")
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        if Y is None:
+            Y = torch.empty((T, H), dtype=t, device=dev)
+        if ids is None:
+            ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        if weights is None:
+            weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        st = L.b200_moe(BF16 if t == torch.bfloat16 else F16, X.data_ptr(), logits.data_ptr(), W13.data_ptr(), W2.data_ptr(), Y.data_ptr(),
+                        ids.data_ptr(), weights.data_ptr(), T, H, I, E, top_k, int(normalise), workspace.data_ptr(),
+                        workspace.numel() * workspace.element_size(), sptr)
+    if st != OK:
+        raise B200Error(st, "b200_moe")
+    return Y, ids, weights
 
 
 def device_status(stream=None):

@@ -112,6 +112,26 @@ int encode_2d(CUtensorMap *map, CUtensorMapDataType type, int elem_bytes, const 
     return B200_OK;
 }
 
+}  // namespace
+
+// For the library's other translation units: the status of the current device (probing it on the first call) and its SM
+// count; a tiled tensor map of a row-major two-byte matrix; the budget of a bounded wait in SM cycles.
+int current_device(int *num_sms) {
+    const DeviceInfo *dev = nullptr;
+    const int st = device_info(&dev);
+    if (st == B200_OK && num_sms) *num_sms = dev->num_sms;
+    return st;
+}
+
+int encode_operand_map(CUtensorMap *map, int dtype, const void *ptr, uint64_t inner, uint64_t outer, uint32_t box_outer) {
+    return encode_2d(map, dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, ptr, inner, outer,
+                     kBoxK, box_outer);
+}
+
+long long wait_budget_cycles() { return static_cast<long long>(g_wait_budget_ns.load() * 2ull); }  // SM clock is below 2 GHz
+
+namespace {
+
 // Tuned defaults. Large problems use the two-CTA pair (256 x 256 tile, each CTA stages 128 rows of
 // A and 128 rows of B^T per K block: half the L2-to-shared traffic per flop of a one-CTA
 // 128 x 256 tile); small or skinny ones a one-CTA tile with the widest N that divides.

@@ -1,0 +1,58 @@
+// Shared pieces of the products whose rows choose their own weights (lora.cu, moe.cu): two-byte element
+// conversions and the host's pointer checks.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "gemm_sm100.cuh"
+
+namespace b200 {
+
+struct Bf16 {
+    static constexpr int kCode = B200_BF16;
+    // two packed elements -> two floats; element 0 sits in the low half
+    __device__ static __forceinline__ float2 unpack(uint32_t v) {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
+    __device__ static __forceinline__ uint16_t round(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+};
+
+struct Fp16 {
+    static constexpr int kCode = B200_F16;
+    __device__ static __forceinline__ float2 unpack(uint32_t v) {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    }
+    __device__ static __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+};
+
+// fp32 dot product of eight packed elements on both sides, added to acc
+template <typename T>
+__device__ __forceinline__ float dot8(const uint4 &a, const uint4 &b, float acc) {
+    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = T::unpack(av[i]), y = T::unpack(bv[i]);
+        acc = fmaf(x.x, y.x, acc);
+        acc = fmaf(x.y, y.y, acc);
+    }
+    return acc;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+inline bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+// whether [a, a + na) and [b, b + nb) share a byte
+inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
+}  // namespace b200

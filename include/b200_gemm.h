@@ -286,6 +286,48 @@ int b200_session_gemm_host_sharded(b200_session *s, int dtype, const void *hA_ro
                                    int rank, void *const *peer_bt, void *const *peer_flags, int epoch,
                                    const b200_gemm_params *p);
 
+/* Products whose rows choose their own weights (decode and prompt steps of a language model). They have no
+ * counterpart in the reference, whose launchers multiply every row of A with the same B. Operands and
+ * outputs are fp16 or bf16 (dtype), sums are fp32, outputs are rounded once. As everywhere here the calls
+ * allocate nothing, enqueue on the given stream and return; the same inputs give the same bits. The workspace
+ * (256-byte aligned, any contents) holds intermediate sums: calls that may overlap on the GPU (two streams,
+ * two graphs replayed side by side) need one each. Outputs must not overlap inputs or the workspace. */
+
+/* A projection shared by all rows with low-rank adapters of many requests beside it:
+ *
+ *     D[i] = A[i] * B^T + lora_scale[s] * (A[i] * lora_a[s]^T) * lora_b[s]^T,   s = row_adapter[i]
+ *
+ * A is m x k, Bt n x k, D m x n (all of dtype); lora_a is num_adapters x rank x k, lora_b num_adapters x n x rank
+ * (of dtype), lora_scale num_adapters floats (null: 1), row_adapter m ints on the device. A row whose entry lies
+ * outside [0, num_adapters) has no adapter. Any order of the entries is allowed; rows of one request
+ * behind one another share their adapter's reads. Adapters of several ranks are stacked at the largest, filled up
+ * with zeros; weights of adapters that no row names are not read. N, K and rank are multiples of 8,
+ * rank <= B200_LORA_MAX_RANK. A null row_adapter is refused; num_adapters = 0 is refused (that is b200_gemm_bf16). */
+enum { B200_LORA_MAX_RANK = 128 };
+int64_t b200_gemm_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank);
+int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D, int64_t M, int64_t N, int64_t K, const void *lora_a,
+                   const void *lora_b, const float *lora_scale, const int *row_adapter, int64_t num_adapters, int rank,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* A whole mixture-of-experts layer for a few tokens (at most B200_MOE_MAX_TOKENS):
+ *
+ *     Y[t] = sum over j of w[t][j] * W2[e] * (silu(G[e] * X[t]) . (U[e] * X[t])),   e = ids[t][j],  silu(z) = z / (1 + exp(-z))
+ *
+ * X and Y are tokens x hidden, W13 is experts x (2 * inner) x hidden with G[e] in the first inner rows of an expert and
+ * U[e] in the others, W2 is experts x hidden x inner (all of dtype); logits is tokens x experts fp32 (the D of
+ * a b200_gemm call is one). The top_k largest logits of a token choose its experts, ties go to the lower index; w is
+ * their softmax (normalise = 1: over the chosen ones; 0: over all of the token's logits). An expert whose logit is
+ * -infinity or NaN is never chosen; where fewer than top_k are left, the other entries of ids are -1 with weight 0, and a
+ * token with none gets a zero row; +infinity counts as the largest finite value. ids (int) and weights (float), both
+ * tokens x top_k in descending order of the logits, are outputs; either may be null. Weights of experts that no
+ * token chose are not read. hidden and inner are multiples of 8, experts <= B200_MOE_MAX_EXPERTS, top_k <=
+ * min(experts, B200_MOE_MAX_TOP_K). */
+enum { B200_MOE_MAX_TOKENS = 256, B200_MOE_MAX_EXPERTS = 512, B200_MOE_MAX_TOP_K = 16 };
+int64_t b200_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k);
+int b200_moe(int dtype, const void *X, const float *logits, const void *W13, const void *W2, void *Y, int *ids, float *weights,
+             int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k, int normalise, void *workspace,
+             size_t workspace_bytes, void *stream);
+
 /* Synchronises the stream and reports whether any kernel of this library hit a bounded-wait
  * timeout on the current device since the last call. info (may be null) receives
  * {code, block, barrier id, phase}. Clears the record. Barrier ids of the GEMM kernel: 100 + stage a producer's
