@@ -33,6 +33,7 @@ struct DeviceInfo {
     int ready = 0;  // 0 = not probed, 1 = usable, -1 = unusable
     int status = B200_UNSUPPORTED_DEVICE;
     int num_sms = 0;
+    int *status_record = nullptr;  // device address of the bounded-wait record
 };
 
 constexpr int kMaxDevices = 64;
@@ -84,7 +85,9 @@ int device_info(const DeviceInfo **out) {
             }
             g_encode = reinterpret_cast<EncodeTiledFn>(fn);
         }
-        const int pe = prepare_kernels();
+        int pe = prepare_kernels();
+        if (pe == 0) pe = prepare_routed_kernels();
+        if (pe == 0) pe = device_status_address(&d.status_record);
         if (pe != 0) {
             d.status = fail_cuda(static_cast<cudaError_t>(pe));
             return d.status;
@@ -114,12 +117,14 @@ int encode_2d(CUtensorMap *map, CUtensorMapDataType type, int elem_bytes, const 
 
 }  // namespace
 
-// For the library's other translation units: the status of the current device (probing it on the first call) and its SM
-// count; a tiled tensor map of a row-major two-byte matrix; the budget of a bounded wait in SM cycles.
-int current_device(int *num_sms) {
+// For the library's other translation units: the status of the current device (probing it on the first call), its SM
+// count and status record; a tiled tensor map of a row-major two-byte matrix; the budget of a bounded wait in SM cycles.
+int current_device(int *num_sms, int **status_record) {
     const DeviceInfo *dev = nullptr;
     const int st = device_info(&dev);
-    if (st == B200_OK && num_sms) *num_sms = dev->num_sms;
+    if (st != B200_OK) return st;
+    if (num_sms) *num_sms = dev->num_sms;
+    if (status_record) *status_record = dev->status_record;
     return st;
 }
 

@@ -1669,6 +1669,10 @@ int launch_splitk_reduce(const float *partial, const float *C, float *D, float a
     return static_cast<int>(cudaGetLastError());
 }
 
+int device_status_address(int **out) {
+    return static_cast<int>(cudaGetSymbolAddress(reinterpret_cast<void **>(out), g_device_status));
+}
+
 int read_device_status(int out[4], cudaStream_t stream) {
     cudaError_t e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return static_cast<int>(e);

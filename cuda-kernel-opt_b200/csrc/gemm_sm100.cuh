@@ -82,11 +82,14 @@ int launch_splitk_reduce_push(const float *partial, int64_t m, int64_t n, int sp
                               unsigned int *done, int world, int rank, int epoch, cudaStream_t stream);
 // Remembers the cudaError_t behind a B200_CUDA_ERROR return for b200_last_cuda_error(); returns B200_CUDA_ERROR.
 int record_cuda_error(int cuda_error);
-// Status of the current device (B200_OK or why it cannot be used), probed on the first call; its SM count.
-int current_device(int *num_sms);
+// Status of the current device (B200_OK or why it cannot be used), probed on the first call; its SM count and the device
+// address of its status record (either may be null).
+int current_device(int *num_sms, int **status_record);
+int device_status_address(int **out);   // cudaError_t as int; what current_device remembers
 // Tensor map of a row-major two-byte matrix {inner, outer}, box {64, box_outer}, 128-byte swizzle.
 int encode_operand_map(CUtensorMap *map, int dtype, const void *ptr, uint64_t inner, uint64_t outer, uint32_t box_outer);
 long long wait_budget_cycles();
+int prepare_routed_kernels();  // the same for lora.cu and moe.cu
 int prepare_kernels();  // opt-in shared memory size; once per device
 int profile_slots();    // int64 slots per CTA of the profile buffer (16; 32 in a -DB200_TIMELINE build)
 

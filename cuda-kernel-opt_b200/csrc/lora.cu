@@ -129,6 +129,10 @@ int check_lora(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) 
 }
 
 }  // namespace
+
+int prepare_moe_kernels();
+int prepare_routed_kernels() { return prepare_moe_kernels(); }
+
 }  // namespace b200
 
 extern "C" int64_t b200_gemm_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) {
@@ -154,7 +158,7 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     for (const auto &i : in)
         if (overlap(D, M * N * 2, i.p, i.n) || overlap(workspace, need, i.p, i.n)) return B200_INVALID_POINTER;
     if (overlap(D, M * N * 2, workspace, need)) return B200_INVALID_POINTER;
-    st = current_device(nullptr);
+    st = current_device(nullptr, nullptr);
     if (st != B200_OK) return st;
     LoraArgs g = {};
     g.A = static_cast<const uint16_t *>(A);

@@ -2,8 +2,24 @@
 //
 //     Y[t] = sum_j w[t][j] W2[e] (silu(G[e] X[t]) . (U[e] X[t])),   e = ids[t][j] = the j-th largest router logit of t
 //
-// Three kernels: the router's choice, the gated product of every (token, choice) slot, the second product
-// with the weighted sum over a token's choices.
+// What bounds it is reading the chosen experts' weights once (3 * inner * hidden two-byte values each): a token
+// more per expert costs almost nothing. So the weights take the 128-row side of tcgen05.mma and the tokens of one expert
+// its N side, and the work (chosen experts x row tiles x K blocks of 64) is cut into one equal, contiguous stretch of K
+// blocks per CTA, wherever that falls: with 8 chosen experts of 96 tiles on 148 SMs whole tiles would leave a third of
+// the SMs idle, and an SM streams at most some 45 GB/s. A tile whose K blocks end up in several CTAs leaves
+// that many partial sums ("parts") in the workspace, which the next kernel adds in ascending order: no CTA waits for
+// another, nothing is accumulated atomically, the same inputs give the same bits.
+//
+//   moe_route_kernel    one block: the choice per token (one warp each), the list of chosen experts with their tokens
+//   moe_product_kernel  <UP>: a tile is 64 rows of G and the same 64 rows of U; parts of both (fp32) to the workspace
+//   moe_product_kernel  <DOWN>: a tile is 128 rows of W2; the loader warps add the parts of a K block, apply silu and the
+//                       gate, and hand the result to the tensor core as a pair of 16-bit numbers, value and remainder
+//                       (two MMAs per K step: the tensor core idles here, and one 16-bit rounding of the gated value
+//                       would cost as much accuracy as the rounding of the result)
+//   moe_combine_kernel  adds the parts and the weighted choices of a token, one rounding
+//
+// The kernels are launched as programmatic dependents: UP lets DOWN start at once, so DOWN's CTAs (two CTAs fit an SM while
+// the tokens are few) fill their ring with weights while UP still runs, and wait only before they read its sums.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -11,21 +27,60 @@
 
 #include "../../include/b200_gemm.h"
 #include "gemm_sm100.cuh"
+#include "pipeline.cuh"
 #include "routed.cuh"
 
 namespace b200 {
 namespace {
 
-struct MoeArgs {
-    const uint16_t *X, *W13, *W2;
+constexpr int kMoeStages = 16;      // most stages of the ring
+constexpr int kMoeLoaders = 8;      // warps that bring the activations of a K block
+constexpr int kMoeThreads = (2 + 4 + kMoeLoaders) * 32;
+constexpr int kMaxParts = 16;
+constexpr int kGridSms = 148;       // what the workspace is sized for; another count only changes how tiles are cut
+constexpr int kWeightBytes = 128 * 128;  // one K block of a weight tile: 128 rows of 64 elements
+
+// What the route kernel leaves for the others, in the workspace.
+struct Lists {
+    int *header;     // [0] chosen experts, [1] most tokens of one
+    int *expert;     // per chosen expert: its index, its number of tokens, the first of its slots
+    int *count;
+    int *base;
+    int *token;      // per slot (sorted by expert, then token): its token
+    int *slot;       // per (token, choice): its slot, -1 without one
+    int *active;     // per (token, choice): the position of its expert in the list of chosen ones
+    float *weight;   // per (token, choice)
+};
+
+struct alignas(64) MoeArgs {
+    CUtensorMap map;          // of the product's weights
+    const uint16_t *X;
     const float *logits;
     uint16_t *Y;
     int *ids_out;
     float *weights_out;
-    int *ids;        // tokens x top_k, workspace
-    float *weights;  // tokens x top_k, workspace
-    float *h;        // tokens x top_k x inner, workspace
-    int tokens, hidden, inner, experts, top_k, normalise;
+    Lists list;
+    float *z;                 // [part][slot][2 * inner]: sums of UP
+    float *o;                 // [part][slot][hidden]: sums of DOWN
+    int tokens, hidden, inner, experts, top_k, normalise, slots;
+    int parts_up, parts_down;
+    int sms;
+    int ring_bytes, off_token, off_expert, off_bars, off_misc;
+    int tmem_cols, slot_cols;
+    uint32_t idesc;           // with N = 0
+    int *status;
+    long long budget;
+};
+
+// How the K blocks of `units` tiles are dealt out: CTA c takes blocks [c * len, (c + 1) * len) of all of them in a row. len is
+// large enough for a tile to touch at most `parts` CTAs.
+struct Cut {
+    int kblocks, total, len;
+    __device__ __forceinline__ Cut(int units, int kblocks_, int sms, int parts) : kblocks(kblocks_), total(units * kblocks_) {
+        len = max(max((total + sms - 1) / sms, (kblocks - 1 + parts - 2) / (parts - 1)), 1);
+    }
+    __device__ __forceinline__ int first_cta(int unit) const { return unit * kblocks / len; }
+    __device__ __forceinline__ int num_parts(int unit) const { return ((unit + 1) * kblocks - 1) / len - first_cta(unit) + 1; }
 };
 
 // Order-preserving map of a logit to an unsigned key; 0 = never chosen (-infinity, NaN). Equal floats (+-0 among
@@ -86,91 +141,428 @@ __device__ __forceinline__ void choose_experts(const float *logits, int experts,
     if (id >= 0) weight /= sum;
 }
 
-__global__ void __launch_bounds__(32) moe_route_kernel(const MoeArgs g) {
-    const int t = blockIdx.x, lane = threadIdx.x;
-    int id;
-    float w;
-    choose_experts(g.logits + static_cast<int64_t>(t) * g.experts, g.experts, g.top_k, g.normalise, lane, id, w);
-    if (lane < g.top_k) {
-        const int at = t * g.top_k + lane;
-        g.ids[at] = id;
-        g.weights[at] = w;
-        if (g.ids_out) g.ids_out[at] = id;
-        if (g.weights_out) g.weights_out[at] = w;
-    }
-}
 
-// One warp per (slot, inner row): both halves' dot products.
-template <typename T>
-__global__ void __launch_bounds__(256) moe_up_kernel(const MoeArgs g) {
-    const int slot = blockIdx.x, lane = threadIdx.x & 31, e = g.ids[slot];
-    if (e < 0) return;
-    const uint4 *x = reinterpret_cast<const uint4 *>(g.X + static_cast<int64_t>(slot / g.top_k) * g.hidden);
-    for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < g.inner; i += gridDim.y * 8) {
-        const uint4 *wg = reinterpret_cast<const uint4 *>(g.W13 + (static_cast<int64_t>(e) * 2 * g.inner + i) * g.hidden);
-        const uint4 *wu = reinterpret_cast<const uint4 *>(g.W13 + (static_cast<int64_t>(e) * 2 * g.inner + g.inner + i) * g.hidden);
-        float a = 0.0f, b = 0.0f;
-        for (int k = lane; k < g.hidden / 8; k += 32) {
-            a = dot8<T>(x[k], wg[k], a);
-            b = dot8<T>(x[k], wu[k], b);
+__global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__ MoeArgs g) {
+    __shared__ uint32_t mask[B200_MOE_MAX_EXPERTS][B200_MOE_MAX_TOKENS / 32];   // the tokens of an expert
+    __shared__ short place[B200_MOE_MAX_EXPERTS];                               // its position among the chosen
+    __shared__ int first[B200_MOE_MAX_EXPERTS];                                 // its first slot
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int words = (g.tokens + 31) / 32;
+    for (int i = tid; i < g.experts * words; i += 1024) mask[i / words][i % words] = 0u;
+    griddep_wait();
+    griddep_launch_dependents();
+    __syncthreads();
+    for (int t = warp; t < g.tokens; t += 32) {
+        int id;
+        float w;
+        choose_experts(g.logits + static_cast<int64_t>(t) * g.experts, g.experts, g.top_k, g.normalise, lane, id, w);
+        if (lane < g.top_k) {
+            const int at = t * g.top_k + lane;
+            g.list.slot[at] = id;       // the expert for now
+            g.list.weight[at] = w;
+            if (g.ids_out) g.ids_out[at] = id;
+            if (g.weights_out) g.weights_out[at] = w;
+            if (id >= 0) atomicOr(&mask[id][t >> 5], 1u << (t & 31));
         }
-        a = warp_sum(a);
-        b = warp_sum(b);
-        if (lane == 0) g.h[static_cast<int64_t>(slot) * g.inner + i] = a / (1.0f + expf(-a)) * b;
     }
-}
-
-// One warp per (token, hidden row): the choices in order.
-template <typename T>
-__global__ void __launch_bounds__(256) moe_down_kernel(const MoeArgs g) {
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    for (int n = blockIdx.y * 8 + (threadIdx.x >> 5); n < g.hidden; n += gridDim.y * 8) {
-        float y = 0.0f;
-        for (int j = 0; j < g.top_k; ++j) {
-            const int slot = t * g.top_k + j, e = g.ids[slot];
-            if (e < 0) continue;
-            const uint4 *w = reinterpret_cast<const uint4 *>(g.W2 + (static_cast<int64_t>(e) * g.hidden + n) * g.inner);
-            const float4 *h = reinterpret_cast<const float4 *>(g.h + static_cast<int64_t>(slot) * g.inner);
-            float acc = 0.0f;
-            for (int k = lane; k < g.inner / 8; k += 32) {
-                const uint4 q = w[k];
-                const float4 h0 = h[2 * k], h1 = h[2 * k + 1];
-                const float2 w0 = T::unpack(q.x), w1 = T::unpack(q.y), w2 = T::unpack(q.z), w3 = T::unpack(q.w);
-                acc = fmaf(h0.x, w0.x, fmaf(h0.y, w0.y, fmaf(h0.z, w1.x, fmaf(h0.w, w1.y, acc))));
-                acc = fmaf(h1.x, w2.x, fmaf(h1.y, w2.y, fmaf(h1.z, w3.x, fmaf(h1.w, w3.y, acc))));
+    __syncthreads();
+    if (warp == 0) {
+        int chosen = 0, slots = 0, most = 0;
+        for (int e0 = 0; e0 < g.experts; e0 += 32) {
+            const int e = e0 + lane;
+            int n = 0;
+            if (e < g.experts)
+                for (int i = 0; i < words; ++i) n += __popc(mask[e][i]);
+            const uint32_t ballot = __ballot_sync(0xffffffffu, n > 0);
+            int before = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
             }
-            y = fmaf(g.weights[slot], warp_sum(acc), y);
+            if (n > 0) {
+                const int at = chosen + __popc(ballot & ((1u << lane) - 1u));
+                g.list.expert[at] = e;
+                g.list.count[at] = n;
+                g.list.base[at] = slots + before - n;
+                place[e] = static_cast<short>(at);
+                first[e] = slots + before - n;
+            }
+            chosen += __popc(ballot);
+            slots += __shfl_sync(0xffffffffu, before, 31);
+            most = max(most, static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(n))));
         }
-        if (lane == 0) g.Y[static_cast<int64_t>(t) * g.hidden + n] = T::round(y);
+        if (lane == 0) {
+            g.list.header[0] = chosen;
+            g.list.header[1] = most;
+        }
+    }
+    __syncthreads();
+    for (int at = tid; at < g.slots; at += 1024) {
+        const int t = at / g.top_k, e = g.list.slot[at];
+        if (e < 0) continue;
+        int slot = first[e] + __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
+        for (int i = 0; i < (t >> 5); ++i) slot += __popc(mask[e][i]);
+        g.list.token[slot] = t;
+        g.list.slot[at] = slot;
+        g.list.active[at] = place[e];
     }
 }
 
+// The stretch of one CTA, cut at tile borders: K blocks [kb0, kb1) of tile `tile` of chosen expert `ai`.
+struct Segment {
+    int ai, tile, kb0, kb1, part;
+};
+
+struct Walker {
+    int q, end, tiles, cta;
+    Cut cut;
+    __device__ __forceinline__ Walker(const Cut &c, int tiles_, int cta_) : tiles(tiles_), cta(cta_), cut(c) {
+        q = min(static_cast<long long>(cta) * c.len, static_cast<long long>(c.total));
+        end = min(q + c.len, c.total);
+    }
+    __device__ __forceinline__ bool next(Segment &s) {
+        if (q >= end) return false;
+        const int unit = q / cut.kblocks;
+        s.ai = unit / tiles;
+        s.tile = unit - s.ai * tiles;
+        s.kb0 = q - unit * cut.kblocks;
+        s.kb1 = min(cut.kblocks, s.kb0 + end - q);
+        s.part = cta - cut.first_cta(unit);
+        q += s.kb1 - s.kb0;
+        return true;
+    }
+};
+
+template <typename T, bool DOWN>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __grid_constant__ MoeArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t ring = (raw + 1023u) & ~1023u;
+    uint8_t *const sm = smem_raw + (ring - raw);
+    uint16_t *const token_s = reinterpret_cast<uint16_t *>(sm + g.off_token);
+    int *const expert_s = reinterpret_cast<int *>(sm + g.off_expert);
+    int *const count_s = expert_s + g.experts, *const base_s = count_s + g.experts;
+    const uint32_t full0 = ring + g.off_bars, empty0 = full0 + 8 * kMoeStages, acc_full0 = empty0 + 8 * kMoeStages, acc_empty0 = acc_full0 + 16;
+    volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // [0] abort flag, [1] tensor-memory base
+    const WaitCtx wait = {g.status, misc, g.budget};
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+
+    if (tid < 2 * kMoeStages + 4) {
+        // full: the producer's byte count and four arrivals of the loader warps; accumulator empty: the four draining warps
+        mbar_init(full0 + 8 * tid, tid < kMoeStages ? 5 : tid < 2 * kMoeStages + 2 ? 1 : 4);
+        fence_mbar_init();
+    }
+    if (tid == 0) misc[0] = 0;
+    if (tid == 32) tma_prefetch_desc(&g.map);
+    if (warp == 1) {
+        tmem_alloc<1>(ring + g.off_misc + 4, g.tmem_cols);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    // UP waits for the route kernel; every CTA of UP says so before DOWN may start, so DOWN finds the lists (and all that came
+    // before the call) complete without a wait of its own, and waits later for UP's sums.
+    if (!DOWN) griddep_wait();
+    griddep_launch_dependents();
+    const int chosen = __ldcg(g.list.header), most = __ldcg(g.list.header + 1);
+    for (int i = tid; i < chosen; i += kMoeThreads) {
+        expert_s[i] = __ldcg(g.list.expert + i);
+        count_s[i] = __ldcg(g.list.count + i);
+        base_s[i] = __ldcg(g.list.base + i);
+    }
+    if (!DOWN)
+        for (int i = tid; i < g.slots; i += kMoeThreads) token_s[i] = static_cast<uint16_t>(__ldcg(g.list.token + i));
+    __syncthreads();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[1]), 0);
+
+    const int tiles_up = (g.inner + 63) / 64, kb_up = (g.hidden + 63) / 64;
+    const int tiles = DOWN ? (g.hidden + 127) / 128 : tiles_up;
+    const Cut cut(chosen * tiles, DOWN ? tiles_up : kb_up, g.sms, DOWN ? g.parts_down : g.parts_up);
+    const uint32_t rows_bytes = static_cast<uint32_t>((most + 15) / 16 * 16 * 128);   // the activations of a K block (16-bit values)
+    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (DOWN ? 2 : 1);
+    const int stages = min(kMoeStages, static_cast<int>(g.ring_bytes / stage_bytes));
+    Walker walk(cut, tiles, blockIdx.x);
+    Segment s;
+    int st = 0;
+    uint32_t ph = 0;
+
+    if (warp == 0) {
+        // -------------------------------------------------------------- weights: TMA
+        const bool issuer = elect_one();
+        const uint64_t once = l2_policy(1);
+        bool ok = true;
+        while (ok && walk.next(s)) {
+            const int e = expert_s[s.ai];
+            const int row = DOWN ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
+            for (int kb = s.kb0; kb < s.kb1; ++kb) {
+                ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1000 + st);
+                if (!ok) break;
+                if (issuer) {
+                    const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
+                    mbar_arrive_expect_tx(bar, kWeightBytes);
+                    tma_load_2d_hint(dst, &g.map, bar, kb * 64, row, once);
+                    if (!DOWN) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
+                }
+                if (++st == stages) st = 0, ph ^= 1u;
+            }
+        }
+    } else if (warp == 1) {
+        // -------------------------------------------------------------- MMA
+        const bool issuer = elect_one();
+        bool ok = true;
+        for (int n = 0; ok && walk.next(s); ++n) {
+            const int acc = n & 1;
+            ok = wait_warp(acc_empty0 + 8 * acc, ((n >> 1) & 1) ^ 1u, wait, 1100 + acc);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t d = tmem + acc * g.slot_cols;
+            const uint32_t idesc = g.idesc | static_cast<uint32_t>((count_s[s.ai] + 15) / 16 * 2) << 17;
+            for (int kb = s.kb0; kb < s.kb1; ++kb) {
+                ok = wait_warp(full0 + 8 * st, ph, wait, 1200 + st);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t at = ring + st * stage_bytes;
+                const uint64_t a = umma_desc_sw128(at), b = umma_desc_sw128(at + kWeightBytes), lo = umma_desc_sw128(at + kWeightBytes + rows_bytes);
+                if (issuer) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        umma_f16<1>(d, a + 2 * i, b + 2 * i, idesc, kb > s.kb0 || i > 0);
+                        if (DOWN) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
+                    }
+                    umma_commit<1>(empty0 + 8 * st);
+                }
+                if (++st == stages) st = 0, ph ^= 1u;
+            }
+            if (ok && issuer) umma_commit<1>(acc_full0 + 8 * acc);
+        }
+        __syncwarp();
+    } else if (warp < 6) {
+        // -------------------------------------------------------------- accumulators -> parts in the workspace
+        const int quarter = warp & 3;
+        const int r = quarter * 32 + lane;                 // row of the tile
+        bool ok = true;
+        if (DOWN) griddep_wait();                          // in every CTA, with work or without: DOWN must not complete before UP
+        for (int n = 0; ok && walk.next(s); ++n) {
+            const int acc = n & 1, count = count_s[s.ai];
+            const int64_t slot = static_cast<int64_t>(s.part) * g.slots + base_s[s.ai];
+            float *out;
+            int pitch;
+            bool mine;
+            if (DOWN) {
+                mine = s.tile * 128 + r < g.hidden;
+                pitch = g.hidden;
+                out = g.o + slot * pitch + s.tile * 128 + r;
+            } else {
+                const int i = s.tile * 64 + (r & 63);
+                mine = i < g.inner;
+                pitch = 2 * g.inner;
+                out = g.z + slot * pitch + (r < 64 ? i : g.inner + i);
+            }
+            ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 1300 + acc);
+            if (!ok) break;
+            tc_fence_after_sync();
+            for (int c = 0; c < count; c += 16) {
+                uint32_t v[16];
+                tmem_ld_32x16(tmem + acc * g.slot_cols + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                tmem_ld_wait();
+                if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < count) out[static_cast<int64_t>(c + j) * pitch] = __uint_as_float(v[j]);
+                }
+                __syncwarp();
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty0 + 8 * acc);
+        }
+    } else {
+        // -------------------------------------------------------------- activations
+        // The loader warps form groups that take the K blocks in turn, so that the latency of a block's loads is spread over
+        // several blocks. A group looks at a stage only when its own turn comes; the phase it waits for cannot be
+        // mistaken for the one two before it as long as there are no more groups than stages.
+        const int group_warps = stages >= 8 ? 1 : stages >= 4 ? 2 : 4, groups = kMoeLoaders / group_warps;
+        const int mine = (warp - 6) / group_warps, chunk = lane & 7;
+        const int row0 = (warp - 6) % group_warps * 4 + (lane >> 3), row_step = 4 * group_warps;
+        const Cut up(chosen * tiles_up, kb_up, g.sms, g.parts_up);
+        const int64_t part_pitch = static_cast<int64_t>(g.slots) * 2 * g.inner;
+        int turn = 0;
+        bool ok = true;
+        if (DOWN) griddep_wait();
+        while (ok && walk.next(s)) {
+            const int count = count_s[s.ai], base = base_s[s.ai];
+            for (int kb = s.kb0; kb < s.kb1; ++kb) {
+                if (turn == mine) {
+                    ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1400 + st);
+                    if (!ok) break;
+                    const uint32_t dst = ring + st * stage_bytes + kWeightBytes;
+                    const int k = kb * 64 + chunk * 8;
+                    if (!DOWN) {
+                        for (int r = row0; r < count; r += row_step) {
+                            if (k < g.hidden) cp_async_16(dst + swizzled(r, chunk), g.X + static_cast<int64_t>(token_s[base + r]) * g.hidden + k);
+                            else st_shared_v4(dst + swizzled(r, chunk), make_uint4(0, 0, 0, 0));
+                        }
+                        cp_async_wait_all();
+                    } else {
+                        const int unit = s.ai * tiles_up + kb, parts = up.num_parts(unit);
+                        for (int r = row0; r < count; r += row_step) {
+                            uint32_t hi[4] = {}, lo[4] = {};
+                            if (k < g.inner) {
+                                const float *z = g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k;
+                                float gate[8] = {}, up8[8] = {};
+                                for (int p = 0; p < parts; ++p, z += part_pitch) {
+                                    const float4 a = __ldcg(reinterpret_cast<const float4 *>(z)), b = __ldcg(reinterpret_cast<const float4 *>(z + 4));
+                                    const float4 c = __ldcg(reinterpret_cast<const float4 *>(z + g.inner)), d = __ldcg(reinterpret_cast<const float4 *>(z + g.inner + 4));
+                                    gate[0] += a.x, gate[1] += a.y, gate[2] += a.z, gate[3] += a.w, gate[4] += b.x, gate[5] += b.y, gate[6] += b.z, gate[7] += b.w;
+                                    up8[0] += c.x, up8[1] += c.y, up8[2] += c.z, up8[3] += c.w, up8[4] += d.x, up8[5] += d.y, up8[6] += d.z, up8[7] += d.w;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    uint16_t h0, h1, l0, l1;
+                                    T::split(__fdividef(gate[2 * i], 1.0f + __expf(-gate[2 * i])) * up8[2 * i], h0, l0);
+                                    T::split(__fdividef(gate[2 * i + 1], 1.0f + __expf(-gate[2 * i + 1])) * up8[2 * i + 1], h1, l1);
+                                    hi[i] = h0 | static_cast<uint32_t>(h1) << 16;
+                                    lo[i] = l0 | static_cast<uint32_t>(l1) << 16;
+                                }
+                            }
+                            st_shared_v4(dst + swizzled(r, chunk), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                            st_shared_v4(dst + rows_bytes + swizzled(r, chunk), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_many(full0 + 8 * st, 4 / group_warps);
+                }
+                if (++turn == groups) turn = 0;
+                if (++st == stages) st = 0, ph ^= 1u;
+            }
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        if (misc[0]) {   // aborted: give copies and MMAs in flight a bounded time to land before the memory goes
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {
+            }
+        }
+        tc_fence_after_sync();
+        tmem_dealloc<1>(tmem, g.tmem_cols);
+    }
+}
+
+// Four columns of one token per thread: parts in ascending order, choices in descending order of their logits.
 template <typename T>
-int launch_moe(const MoeArgs &g, cudaStream_t stream) {
-    moe_route_kernel<<<g.tokens, 32, 0, stream>>>(g);
-    moe_up_kernel<T><<<dim3(g.tokens * g.top_k, (g.inner + 31) / 32), 256, 0, stream>>>(g);
-    moe_down_kernel<T><<<dim3(g.tokens, (g.hidden + 31) / 32), 256, 0, stream>>>(g);
-    const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? record_cuda_error(e) : B200_OK;
+__global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ MoeArgs g) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t = blockIdx.y, n = (blockIdx.x * 128 + threadIdx.x) * 4;
+    if (n >= g.hidden) return;
+    const int tiles = (g.hidden + 127) / 128;
+    const Cut cut(g.list.header[0] * tiles, (g.inner + 63) / 64, g.sms, g.parts_down);
+    const int64_t pitch = static_cast<int64_t>(g.slots) * g.hidden;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < g.top_k; ++j) {
+        const int at = t * g.top_k + j, slot = g.list.slot[at];
+        if (slot < 0) continue;
+        const int parts = cut.num_parts(g.list.active[at] * tiles + n / 128);
+        const float *o = g.o + static_cast<int64_t>(slot) * g.hidden + n;
+        float4 v = *reinterpret_cast<const float4 *>(o);
+        for (int p = 1; p < parts; ++p) {
+            const float4 u = *reinterpret_cast<const float4 *>(o + p * pitch);
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        const float w = g.list.weight[at];
+        y.x = fmaf(w, v.x, y.x), y.y = fmaf(w, v.y, y.y), y.z = fmaf(w, v.z, y.z), y.w = fmaf(w, v.w, y.w);
+    }
+    uint2 out;
+    out.x = T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16;
+    out.y = T::round(y.z) | static_cast<uint32_t>(T::round(y.w)) << 16;
+    *reinterpret_cast<uint2 *>(g.Y + static_cast<int64_t>(t) * g.hidden + n) = out;
 }
 
 int check_moe(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
     if (tokens <= 0 || tokens > B200_MOE_MAX_TOKENS || hidden <= 0 || inner <= 0 || hidden % 8 || inner % 8) return B200_INVALID_SHAPE;
-    if (hidden > (1 << 20) || inner > (1 << 20) || experts <= 0 || experts > B200_MOE_MAX_EXPERTS) return B200_INVALID_SHAPE;
+    if (hidden > 65536 || inner > 65536 || experts <= 0 || experts > B200_MOE_MAX_EXPERTS) return B200_INVALID_SHAPE;
     if (top_k < 1 || top_k > B200_MOE_MAX_TOP_K || top_k > experts) return B200_INVALID_CONFIG;
     return B200_OK;
 }
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// CTAs that may share a tile: what the cut needs when every token chooses the same experts, and one more for stretches that
+// do not start at a tile. Fewer experts than that (masked logits) are cut more coarsely than they could be.
+int most_parts(int64_t units, int64_t kblocks) {
+    const int64_t len = (units * kblocks + kGridSms - 1) / kGridSms;
+    const int64_t parts = (kblocks - 1 + len - 1) / len + 1;
+    return static_cast<int>(parts < 2 ? 2 : parts > kMaxParts ? kMaxParts : parts);
+}
+
+struct MoeLayout {
+    int parts_up, parts_down;
+    int64_t off_list, off_z, off_o, bytes;
+};
+
+MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
+    MoeLayout l;
+    const int64_t slots = tokens * top_k, up_tiles = (inner + 63) / 64;
+    l.parts_up = most_parts(top_k * up_tiles, (hidden + 63) / 64);
+    l.parts_down = most_parts(top_k * ((hidden + 127) / 128), up_tiles);
+    l.off_list = 0;
+    l.off_z = up256((2 + 3 * experts + 4 * slots) * 4);
+    l.off_o = l.off_z + up256(l.parts_up * slots * 2 * inner * 4);
+    l.bytes = l.off_o + up256(l.parts_down * slots * hidden * 4);
+    return l;
+}
+
+template <typename T>
+cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, int smem, cudaStream_t stream) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(1024);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, moe_route_kernel, g);
+    cfg.gridDim = dim3(g.sms);
+    cfg.blockDim = dim3(kMoeThreads);
+    cfg.dynamicSmemBytes = smem;
+    g.map = up;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, false>, g);
+    g.map = down;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, true>, g);
+    cfg.gridDim = dim3((g.hidden + 511) / 512, g.tokens);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_combine_kernel<T>, g);
+    return e;
+}
+
 }  // namespace
+
+int prepare_moe_kernels() {
+    const void *const kernels[] = {reinterpret_cast<const void *>(moe_product_kernel<Bf16, false>), reinterpret_cast<const void *>(moe_product_kernel<Bf16, true>),
+                                   reinterpret_cast<const void *>(moe_product_kernel<Fp16, false>), reinterpret_cast<const void *>(moe_product_kernel<Fp16, true>)};
+    for (const void *k : kernels) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    return 0;
+}
+
 }  // namespace b200
 
 extern "C" int64_t b200_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
     if (b200::check_moe(tokens, hidden, inner, experts, top_k) != B200_OK) return -1;
-    return 2 * b200::up256(tokens * top_k * 4) + tokens * top_k * inner * 4;
+    return b200::moe_layout(tokens, hidden, inner, experts, top_k).bytes;
 }
-
 extern "C" int b200_moe(int dtype, const void *X, const float *logits, const void *W13, const void *W2, void *Y, int *ids, float *weights,
                         int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k, int normalise, void *workspace,
                         size_t workspace_bytes, void *stream) {
@@ -194,26 +586,55 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
         for (int p = 0; p < o; ++p)
             if (overlap(out[o].p, out[o].n, out[p].p, out[p].n)) return B200_INVALID_POINTER;
     }
-    st = current_device(nullptr);
-    if (st != B200_OK) return st;
     MoeArgs g = {};
+    st = current_device(&g.sms, &g.status);
+    if (st != B200_OK) return st;
+    CUtensorMap up, down;
+    st = encode_operand_map(&up, dtype, W13, hidden, experts * 2 * inner, 64);
+    if (st == B200_OK) st = encode_operand_map(&down, dtype, W2, inner, experts * hidden, 128);
+    if (st != B200_OK) return st;
+    const MoeLayout l = moe_layout(tokens, hidden, inner, experts, top_k);
+    uint8_t *const ws = static_cast<uint8_t *>(workspace);
+    const int64_t slots = tokens * top_k;
+    int *const list = reinterpret_cast<int *>(ws + l.off_list);
+    g.list.header = list;
+    g.list.expert = list + 2;
+    g.list.count = g.list.expert + experts;
+    g.list.base = g.list.count + experts;
+    g.list.token = g.list.base + experts;
+    g.list.slot = g.list.token + slots;
+    g.list.active = g.list.slot + slots;
+    g.list.weight = reinterpret_cast<float *>(g.list.active + slots);
+    g.z = reinterpret_cast<float *>(ws + l.off_z);
+    g.o = reinterpret_cast<float *>(ws + l.off_o);
     g.X = static_cast<const uint16_t *>(X);
-    g.W13 = static_cast<const uint16_t *>(W13);
-    g.W2 = static_cast<const uint16_t *>(W2);
     g.logits = logits;
     g.Y = static_cast<uint16_t *>(Y);
     g.ids_out = ids;
     g.weights_out = weights;
-    uint8_t *const ws = static_cast<uint8_t *>(workspace);
-    const int64_t slot_bytes = up256(tokens * top_k * 4);
-    g.ids = reinterpret_cast<int *>(ws);
-    g.weights = reinterpret_cast<float *>(ws + slot_bytes);
-    g.h = reinterpret_cast<float *>(ws + 2 * slot_bytes);
     g.tokens = static_cast<int>(tokens);
     g.hidden = static_cast<int>(hidden);
     g.inner = static_cast<int>(inner);
     g.experts = static_cast<int>(experts);
     g.top_k = top_k;
     g.normalise = normalise;
-    return dtype == B200_BF16 ? launch_moe<Bf16>(g, static_cast<cudaStream_t>(stream)) : launch_moe<Fp16>(g, static_cast<cudaStream_t>(stream));
+    g.slots = static_cast<int>(slots);
+    g.parts_up = l.parts_up;
+    g.parts_down = l.parts_down;
+    // Two accumulators of up to `tokens` columns. While the tokens are few a CTA takes less than half of an SM's shared memory,
+    // so that DOWN can start beside UP; more tokens need the larger ring (a K block of DOWN is up to 80 KB then).
+    g.slot_cols = static_cast<int>((tokens + 15) / 16 * 16);
+    g.tmem_cols = pow2_at_least(2 * g.slot_cols);
+    const int lists = static_cast<int>(up256(slots * 2) + up256(experts * 12));
+    const int smem = tokens <= 16 ? 113 * 1024 : kSmemLimit;
+    g.ring_bytes = (smem - 1024 - lists - 512) / 1024 * 1024;
+    g.off_token = g.ring_bytes;
+    g.off_expert = g.off_token + static_cast<int>(up256(slots * 2));
+    g.off_bars = g.ring_bytes + lists;
+    g.off_misc = g.off_bars + (2 * kMoeStages + 4) * 8;
+    g.idesc = umma_idesc(128, 0, dtype == B200_BF16);
+    g.budget = wait_budget_cycles();
+    const cudaError_t e = dtype == B200_BF16 ? launch_moe<Bf16>(g, up, down, smem, static_cast<cudaStream_t>(stream))
+                                             : launch_moe<Fp16>(g, up, down, smem, static_cast<cudaStream_t>(stream));
+    return e != cudaSuccess ? record_cuda_error(e) : B200_OK;
 }

@@ -18,6 +18,12 @@ struct Bf16 {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     }
     __device__ static __forceinline__ uint16_t round(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+    // v as the sum of two elements. The first one saturates, so that infinities (and what the pair cannot hold) arrive as
+    // an infinity in the second one, not as infinity minus infinity.
+    __device__ static __forceinline__ void split(float v, uint16_t &hi, uint16_t &lo) {
+        hi = round(fminf(fmaxf(v, -3.38953139e38f), 3.38953139e38f));
+        lo = round(v - __uint_as_float(static_cast<uint32_t>(hi) << 16));
+    }
 };
 
 struct Fp16 {
@@ -26,6 +32,10 @@ struct Fp16 {
         return __half22float2(*reinterpret_cast<const __half2 *>(&v));
     }
     __device__ static __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+    __device__ static __forceinline__ void split(float v, uint16_t &hi, uint16_t &lo) {
+        hi = round(fminf(fmaxf(v, -65504.0f), 65504.0f));
+        lo = round(v - __half2float(__ushort_as_half(hi)));
+    }
 };
 
 // fp32 dot product of eight packed elements on both sides, added to acc
