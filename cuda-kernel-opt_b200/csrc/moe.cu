@@ -37,7 +37,9 @@ constexpr int kMoeStages = 16;      // most stages of the ring
 constexpr int kMoeLoaders = 8;      // warps that bring the activations of a K block
 constexpr int kMoeThreads = (2 + 4 + kMoeLoaders) * 32;
 constexpr int kMaxParts = 16;
+constexpr int kFewTokens = 16;      // up to here the loader warps of DOWN compute the gated values, beyond a kernel does
 constexpr int kGridSms = 148;       // what the workspace is sized for; another count only changes how tiles are cut
+constexpr int kBoxBytes = 16 * 128;      // 16 slots of 64 gated values
 constexpr int kWeightBytes = 128 * 128;  // one K block of a weight tile: 128 rows of 64 elements
 
 // What the route kernel leaves for the others, in the workspace.
@@ -54,6 +56,7 @@ struct Lists {
 
 struct alignas(64) MoeArgs {
     CUtensorMap map;          // of the product's weights
+    CUtensorMap map_h;        // of h
     const uint16_t *X;
     const float *logits;
     uint16_t *Y;
@@ -62,6 +65,7 @@ struct alignas(64) MoeArgs {
     Lists list;
     float *z;                 // [part][slot][2 * inner]: sums of UP
     float *o;                 // [part][slot][hidden]: sums of DOWN
+    uint16_t *h;              // [value, remainder][slot][inner]: gated values
     int tokens, hidden, inner, experts, top_k, normalise, slots;
     int parts_up, parts_down;
     int sms;
@@ -93,79 +97,88 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 }
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
 
-// One warp, one token: the top_k largest keys in descending order, ties to the lower index; lane j < top_k returns
-// choice j (id -1, weight 0 where no expert is left).
+// One warp, one token, up to 32 * PER experts: the top_k largest keys in descending order, ties to the lower index; lane
+// j < top_k returns choice j (id -1, weight 0 where no expert is left). A lane keeps its own largest key, so a step is
+// two warp reductions and only the winning lane looks through its keys again.
+template <int PER>
 __device__ __forceinline__ void choose_experts(const float *logits, int experts, int top_k, int normalise, int lane, int &id, float &weight) {
-    constexpr int kPer = B200_MOE_MAX_EXPERTS / 32;
-    uint32_t key[kPer];
+    uint32_t key[PER];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const int e = lane + 32 * i;
         key[i] = e < experts ? logit_key(__ldcg(logits + e)) : 0u;
     }
     uint32_t best = 0u;
+    int best_i = 0;
+    auto look = [&] {
+        best = 0u;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
+        for (int i = 0; i < PER; ++i)
+            if (key[i] > best) best = key[i], best_i = i;
+    };
+    look();
     const float top = key_logit(__reduce_max_sync(0xffffffffu, best));
     float sum = 0.0f;
     if (!normalise) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
+        for (int i = 0; i < PER; ++i)
             if (key[i]) sum += expf(key_logit(key[i]) - top);
         sum = warp_sum(sum);
     }
     id = -1;
-    weight = 0.0f;
+    uint32_t chosen = 0u;
     for (int j = 0; j < top_k; ++j) {
-        uint32_t k = 0u;
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (key[i] > k) {
-                k = key[i];
-                at = lane + 32 * i;
-            }
-        const uint32_t most = __reduce_max_sync(0xffffffffu, k);
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
         if (most == 0u) break;
-        const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(k == most ? at : 0x7fffffff)));
+        const uint32_t e = __reduce_min_sync(0xffffffffu, best == most ? static_cast<uint32_t>(lane + 32 * best_i) : 0xffffffffu);
+        if (lane == static_cast<int>(e & 31u)) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (e == lane + 32 * i) key[i] = 0u;
-        const float w = expf(key_logit(most) - top);
-        if (normalise) sum += w;
-        if (lane == j) {
-            id = e;
-            weight = w;
+            for (int i = 0; i < PER; ++i)
+                if (i == best_i) key[i] = 0u;
+            look();
         }
+        if (lane == j) id = static_cast<int>(e), chosen = most;
     }
+    weight = id >= 0 ? expf(key_logit(chosen) - top) : 0.0f;
+    if (normalise) sum = warp_sum(weight);
     if (id >= 0) weight /= sum;
 }
 
-
+// One cluster of up to eight blocks, a warp per token; its first block then lists the chosen experts and their tokens.
 __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__ MoeArgs g) {
-    __shared__ uint32_t mask[B200_MOE_MAX_EXPERTS][B200_MOE_MAX_TOKENS / 32];   // the tokens of an expert
+    __shared__ uint32_t mask[B200_MOE_MAX_EXPERTS][B200_MOE_MAX_TOKENS / 32];   // the tokens of an expert (of the first block)
     __shared__ short place[B200_MOE_MAX_EXPERTS];                               // its position among the chosen
     __shared__ int first[B200_MOE_MAX_EXPERTS];                                 // its first slot
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int words = (g.tokens + 31) / 32;
-    for (int i = tid; i < g.experts * words; i += 1024) mask[i / words][i % words] = 0u;
+    if (blockIdx.x == 0)
+        for (int i = tid; i < g.experts * words; i += 1024) mask[i / words][i % words] = 0u;
+    cluster_arrive();
     griddep_wait();
     griddep_launch_dependents();
-    __syncthreads();
-    for (int t = warp; t < g.tokens; t += 32) {
-        int id;
-        float w;
-        choose_experts(g.logits + static_cast<int64_t>(t) * g.experts, g.experts, g.top_k, g.normalise, lane, id, w);
-        if (lane < g.top_k) {
-            const int at = t * g.top_k + lane;
-            g.list.slot[at] = id;       // the expert for now
-            g.list.weight[at] = w;
-            if (g.ids_out) g.ids_out[at] = id;
-            if (g.weights_out) g.weights_out[at] = w;
-            if (id >= 0) atomicOr(&mask[id][t >> 5], 1u << (t & 31));
-        }
+    const int t = blockIdx.x * 32 + warp;
+    int id = -1;
+    float w = 0.0f;
+    if (t < g.tokens) {
+        const float *const row = g.logits + static_cast<int64_t>(t) * g.experts;
+        if (g.experts <= 32) choose_experts<1>(row, g.experts, g.top_k, g.normalise, lane, id, w);
+        else if (g.experts <= 64) choose_experts<2>(row, g.experts, g.top_k, g.normalise, lane, id, w);
+        else if (g.experts <= 128) choose_experts<4>(row, g.experts, g.top_k, g.normalise, lane, id, w);
+        else if (g.experts <= 256) choose_experts<8>(row, g.experts, g.top_k, g.normalise, lane, id, w);
+        else choose_experts<16>(row, g.experts, g.top_k, g.normalise, lane, id, w);
     }
-    __syncthreads();
+    cluster_wait();                                         // the first block's masks are zero
+    if (t < g.tokens && lane < g.top_k) {
+        const int at = t * g.top_k + lane;
+        g.list.slot[at] = id;                               // the expert for now
+        g.list.weight[at] = w;
+        if (g.ids_out) g.ids_out[at] = id;
+        if (g.weights_out) g.weights_out[at] = w;
+        if (id >= 0) red_or_cluster(mapa_shared(smem_u32(&mask[id][t >> 5]), 0), 1u << (t & 31));
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (blockIdx.x != 0) return;
     if (warp == 0) {
         int chosen = 0, slots = 0, most = 0;
         for (int e0 = 0; e0 < g.experts; e0 += 32) {
@@ -199,7 +212,7 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__
     }
     __syncthreads();
     for (int at = tid; at < g.slots; at += 1024) {
-        const int t = at / g.top_k, e = g.list.slot[at];
+        const int t = at / g.top_k, e = __ldcg(g.list.slot + at);
         if (e < 0) continue;
         int slot = first[e] + __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
         for (int i = 0; i < (t >> 5); ++i) slot += __popc(mask[e][i]);
@@ -234,7 +247,34 @@ struct Walker {
     }
 };
 
-template <typename T, bool DOWN>
+enum Product {
+    UP,           // gate and up rows times the tokens of X, gathered by the loader warps
+    DOWN_INLINE,  // W2 times the gated values, which the loader warps compute from UP's parts
+    DOWN          // W2 times the gated values that moe_gate_kernel has left in the workspace, by TMA
+};
+
+// The gated value of eight neighbouring inner rows of one slot from UP's parts (ascending), as pairs of 16-bit numbers.
+// The exponential and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th of an fp16.
+template <typename T>
+__device__ __forceinline__ void gated_values(const float *z, int inner, int parts, int64_t part_pitch, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    float gate[8] = {}, up[8] = {};
+    for (int p = 0; p < parts; ++p, z += part_pitch) {
+        const float4 a = __ldcg(reinterpret_cast<const float4 *>(z)), b = __ldcg(reinterpret_cast<const float4 *>(z + 4));
+        const float4 c = __ldcg(reinterpret_cast<const float4 *>(z + inner)), d = __ldcg(reinterpret_cast<const float4 *>(z + inner + 4));
+        gate[0] += a.x, gate[1] += a.y, gate[2] += a.z, gate[3] += a.w, gate[4] += b.x, gate[5] += b.y, gate[6] += b.z, gate[7] += b.w;
+        up[0] += c.x, up[1] += c.y, up[2] += c.z, up[3] += c.w, up[4] += d.x, up[5] += d.y, up[6] += d.z, up[7] += d.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint16_t h0, h1, l0, l1;
+        T::split(__fdividef(gate[2 * i], 1.0f + __expf(-gate[2 * i])) * up[2 * i], h0, l0);
+        T::split(__fdividef(gate[2 * i + 1], 1.0f + __expf(-gate[2 * i + 1])) * up[2 * i + 1], h1, l1);
+        hi[i] = h0 | static_cast<uint32_t>(h1) << 16;
+        lo[i] = l0 | static_cast<uint32_t>(l1) << 16;
+    }
+}
+
+template <typename T, Product P>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __grid_constant__ MoeArgs g) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -251,11 +291,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
 
     if (tid < 2 * kMoeStages + 4) {
         // full: the producer's byte count and four arrivals of the loader warps; accumulator empty: the four draining warps
-        mbar_init(full0 + 8 * tid, tid < kMoeStages ? 5 : tid < 2 * kMoeStages + 2 ? 1 : 4);
+        mbar_init(full0 + 8 * tid, tid < kMoeStages ? (P == DOWN ? 1 : 5) : tid < 2 * kMoeStages + 2 ? 1 : 4);
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0;
     if (tid == 32) tma_prefetch_desc(&g.map);
+    if (P == DOWN && tid == 64) tma_prefetch_desc(&g.map_h);
     if (warp == 1) {
         tmem_alloc<1>(ring + g.off_misc + 4, g.tmem_cols);
         tmem_relinquish<1>();
@@ -265,7 +306,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     tc_fence_after_sync();
     // UP waits for the route kernel; every CTA of UP says so before DOWN may start, so DOWN finds the lists (and all that came
     // before the call) complete without a wait of its own, and waits later for UP's sums.
-    if (!DOWN) griddep_wait();
+    if (P == UP) griddep_wait();
     griddep_launch_dependents();
     const int chosen = __ldcg(g.list.header), most = __ldcg(g.list.header + 1);
     for (int i = tid; i < chosen; i += kMoeThreads) {
@@ -273,16 +314,16 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         count_s[i] = __ldcg(g.list.count + i);
         base_s[i] = __ldcg(g.list.base + i);
     }
-    if (!DOWN)
+    if (P == UP)
         for (int i = tid; i < g.slots; i += kMoeThreads) token_s[i] = static_cast<uint16_t>(__ldcg(g.list.token + i));
     __syncthreads();
     const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[1]), 0);
 
     const int tiles_up = (g.inner + 63) / 64, kb_up = (g.hidden + 63) / 64;
-    const int tiles = DOWN ? (g.hidden + 127) / 128 : tiles_up;
-    const Cut cut(chosen * tiles, DOWN ? tiles_up : kb_up, g.sms, DOWN ? g.parts_down : g.parts_up);
+    const int tiles = P != UP ? (g.hidden + 127) / 128 : tiles_up;
+    const Cut cut(chosen * tiles, P != UP ? tiles_up : kb_up, g.sms, P != UP ? g.parts_down : g.parts_up);
     const uint32_t rows_bytes = static_cast<uint32_t>((most + 15) / 16 * 16 * 128);   // the activations of a K block (16-bit values)
-    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (DOWN ? 2 : 1);
+    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (P != UP ? 2 : 1);
     const int stages = min(kMoeStages, static_cast<int>(g.ring_bytes / stage_bytes));
     Walker walk(cut, tiles, blockIdx.x);
     Segment s;
@@ -294,17 +335,44 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         const bool issuer = elect_one();
         const uint64_t once = l2_policy(1);
         bool ok = true;
+        Walker ahead = walk;
+        Segment f;
+        int fst = 0, fkb = 0, filled = 0;
+        if (P == DOWN) {
+            // the weights of the first stages do not depend on the kernels before: on their way before the wait
+            while (filled < stages && ahead.next(f)) {
+                const int row = expert_s[f.ai] * g.hidden + f.tile * 128;
+                for (fkb = f.kb0; fkb < f.kb1 && filled < stages; ++fkb, ++filled, ++fst)
+                    if (issuer) {
+                        mbar_arrive_expect_tx(full0 + 8 * fst, kWeightBytes + (count_s[f.ai] + 15) / 16 * 2 * kBoxBytes);
+                        tma_load_2d_hint(ring + fst * stage_bytes, &g.map, full0 + 8 * fst, fkb * 64, row, once);
+                    }
+            }
+            griddep_wait();
+        }
         while (ok && walk.next(s)) {
             const int e = expert_s[s.ai];
-            const int row = DOWN ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
+            const int boxes = (count_s[s.ai] + 15) / 16;
+            const int row = P != UP ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
-                ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1000 + st);
-                if (!ok) break;
-                if (issuer) {
-                    const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
-                    mbar_arrive_expect_tx(bar, kWeightBytes);
-                    tma_load_2d_hint(dst, &g.map, bar, kb * 64, row, once);
-                    if (!DOWN) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
+                if (P == DOWN && filled > 0) {
+                    --filled;                              // its weights are on their way
+                } else {
+                    ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1000 + st);
+                    if (!ok) break;
+                    if (issuer) {
+                        const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
+                        mbar_arrive_expect_tx(bar, kWeightBytes + (P == DOWN ? boxes * 2 * kBoxBytes : 0));
+                        tma_load_2d_hint(dst, &g.map, bar, kb * 64, row, once);
+                        if (P == UP) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
+                    }
+                }
+                if (P == DOWN && issuer) {
+                    const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes + kWeightBytes;
+                    for (int b = 0; b < boxes; ++b) {
+                        tma_load_2d(dst + b * kBoxBytes, &g.map_h, bar, kb * 64, base_s[s.ai] + 16 * b);
+                        tma_load_2d(dst + rows_bytes + b * kBoxBytes, &g.map_h, bar, kb * 64, g.slots + base_s[s.ai] + 16 * b);
+                    }
                 }
                 if (++st == stages) st = 0, ph ^= 1u;
             }
@@ -330,7 +398,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         umma_f16<1>(d, a + 2 * i, b + 2 * i, idesc, kb > s.kb0 || i > 0);
-                        if (DOWN) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
+                        if (P != UP) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
                     }
                     umma_commit<1>(empty0 + 8 * st);
                 }
@@ -344,14 +412,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         const int quarter = warp & 3;
         const int r = quarter * 32 + lane;                 // row of the tile
         bool ok = true;
-        if (DOWN) griddep_wait();                          // in every CTA, with work or without: DOWN must not complete before UP
+        if (P != UP) griddep_wait();                          // in every CTA, with work or without: DOWN must not complete before UP
         for (int n = 0; ok && walk.next(s); ++n) {
             const int acc = n & 1, count = count_s[s.ai];
             const int64_t slot = static_cast<int64_t>(s.part) * g.slots + base_s[s.ai];
             float *out;
             int pitch;
             bool mine;
-            if (DOWN) {
+            if (P != UP) {
                 mine = s.tile * 128 + r < g.hidden;
                 pitch = g.hidden;
                 out = g.o + slot * pitch + s.tile * 128 + r;
@@ -379,7 +447,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty0 + 8 * acc);
         }
-    } else {
+    } else if (P != DOWN) {
         // -------------------------------------------------------------- activations
         // The loader warps form groups that take the K blocks in turn, so that the latency of a block's loads is spread over
         // several blocks. A group looks at a stage only when its own turn comes; the phase it waits for cannot be
@@ -391,7 +459,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         const int64_t part_pitch = static_cast<int64_t>(g.slots) * 2 * g.inner;
         int turn = 0;
         bool ok = true;
-        if (DOWN) griddep_wait();
+        if (P != UP) griddep_wait();
         while (ok && walk.next(s)) {
             const int count = count_s[s.ai], base = base_s[s.ai];
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
@@ -400,7 +468,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                     if (!ok) break;
                     const uint32_t dst = ring + st * stage_bytes + kWeightBytes;
                     const int k = kb * 64 + chunk * 8;
-                    if (!DOWN) {
+                    if (P == UP) {
                         for (int r = row0; r < count; r += row_step) {
                             if (k < g.hidden) cp_async_16(dst + swizzled(r, chunk), g.X + static_cast<int64_t>(token_s[base + r]) * g.hidden + k);
                             else st_shared_v4(dst + swizzled(r, chunk), make_uint4(0, 0, 0, 0));
@@ -410,24 +478,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                         const int unit = s.ai * tiles_up + kb, parts = up.num_parts(unit);
                         for (int r = row0; r < count; r += row_step) {
                             uint32_t hi[4] = {}, lo[4] = {};
-                            if (k < g.inner) {
-                                const float *z = g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k;
-                                float gate[8] = {}, up8[8] = {};
-                                for (int p = 0; p < parts; ++p, z += part_pitch) {
-                                    const float4 a = __ldcg(reinterpret_cast<const float4 *>(z)), b = __ldcg(reinterpret_cast<const float4 *>(z + 4));
-                                    const float4 c = __ldcg(reinterpret_cast<const float4 *>(z + g.inner)), d = __ldcg(reinterpret_cast<const float4 *>(z + g.inner + 4));
-                                    gate[0] += a.x, gate[1] += a.y, gate[2] += a.z, gate[3] += a.w, gate[4] += b.x, gate[5] += b.y, gate[6] += b.z, gate[7] += b.w;
-                                    up8[0] += c.x, up8[1] += c.y, up8[2] += c.z, up8[3] += c.w, up8[4] += d.x, up8[5] += d.y, up8[6] += d.z, up8[7] += d.w;
-                                }
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    uint16_t h0, h1, l0, l1;
-                                    T::split(__fdividef(gate[2 * i], 1.0f + __expf(-gate[2 * i])) * up8[2 * i], h0, l0);
-                                    T::split(__fdividef(gate[2 * i + 1], 1.0f + __expf(-gate[2 * i + 1])) * up8[2 * i + 1], h1, l1);
-                                    hi[i] = h0 | static_cast<uint32_t>(h1) << 16;
-                                    lo[i] = l0 | static_cast<uint32_t>(l1) << 16;
-                                }
-                            }
+                            if (k < g.inner) gated_values<T>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k, g.inner, parts, part_pitch, hi, lo);
                             st_shared_v4(dst + swizzled(r, chunk), make_uint4(hi[0], hi[1], hi[2], hi[3]));
                             st_shared_v4(dst + rows_bytes + swizzled(r, chunk), make_uint4(lo[0], lo[1], lo[2], lo[3]));
                         }
@@ -455,29 +506,72 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     }
 }
 
-// Four columns of one token per thread: parts in ascending order, choices in descending order of their logits.
+// The gated values for DOWN: eight inner rows of one slot per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
+    griddep_launch_dependents();   // DOWN reads nothing of this kernel before its own wait
+    griddep_wait();
+    const int chunks = g.inner / 8, tiles = (g.inner + 63) / 64;
+    const int at = blockIdx.x * 256 + threadIdx.x, slot = at / chunks, k = (at - slot * chunks) * 8;
+    const int chosen = __ldcg(g.list.header);
+    if (slot >= g.slots || chosen == 0) return;
+    // the expert of a slot: the last one whose first slot is not behind it
+    int lo_ai = 0, hi_ai = chosen - 1;
+    while (lo_ai < hi_ai) {
+        const int mid = (lo_ai + hi_ai + 1) >> 1;
+        if (__ldcg(g.list.base + mid) <= slot) lo_ai = mid;
+        else hi_ai = mid - 1;
+    }
+    if (slot >= __ldcg(g.list.base + lo_ai) + __ldcg(g.list.count + lo_ai)) return;
+    const Cut up(chosen * tiles, (g.hidden + 63) / 64, g.sms, g.parts_up);
+    uint32_t hi[4], lo[4];
+    gated_values<T>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(lo_ai * tiles + k / 64),
+                    static_cast<int64_t>(g.slots) * 2 * g.inner, hi, lo);
+    *reinterpret_cast<uint4 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// One warp per 128 columns of one token, four per lane: the weighted parts, in ascending order within a choice, choices in
+// descending order of their logits. The warp first lists where they are, so that eight loads are in flight at a time.
 template <typename T>
 __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ MoeArgs g) {
+    __shared__ int2 entry[4][B200_MOE_MAX_TOP_K * kMaxParts];
+    const int t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x * 4 + warp, n = tile * 128 + lane * 4;
+    const int tiles = (g.hidden + 127) / 128;
     griddep_wait();
     griddep_launch_dependents();
-    const int t = blockIdx.y, n = (blockIdx.x * 128 + threadIdx.x) * 4;
+    int slot = -1, parts = 0;
+    float w = 0.0f;
+    if (lane < g.top_k) {
+        const Cut cut(__ldcg(g.list.header) * tiles, (g.inner + 63) / 64, g.sms, g.parts_down);
+        const int at = t * g.top_k + lane;
+        slot = __ldcg(g.list.slot + at);
+        w = __ldcg(g.list.weight + at);
+        if (slot >= 0 && tile < tiles) parts = cut.num_parts(__ldcg(g.list.active + at) * tiles + tile);
+    }
+    int before = parts;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, 31);
+    for (int p = 0; p < parts; ++p) entry[warp][before - parts + p] = make_int2(p * g.slots + slot, __float_as_int(w));
+    __syncwarp();
     if (n >= g.hidden) return;
-    const int tiles = (g.hidden + 127) / 128;
-    const Cut cut(g.list.header[0] * tiles, (g.inner + 63) / 64, g.sms, g.parts_down);
-    const int64_t pitch = static_cast<int64_t>(g.slots) * g.hidden;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int j = 0; j < g.top_k; ++j) {
-        const int at = t * g.top_k + j, slot = g.list.slot[at];
-        if (slot < 0) continue;
-        const int parts = cut.num_parts(g.list.active[at] * tiles + n / 128);
-        const float *o = g.o + static_cast<int64_t>(slot) * g.hidden + n;
-        float4 v = *reinterpret_cast<const float4 *>(o);
-        for (int p = 1; p < parts; ++p) {
-            const float4 u = *reinterpret_cast<const float4 *>(o + p * pitch);
-            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-        }
-        const float w = g.list.weight[at];
-        y.x = fmaf(w, v.x, y.x), y.y = fmaf(w, v.y, y.y), y.z = fmaf(w, v.z, y.z), y.w = fmaf(w, v.w, y.w);
+    for (int i0 = 0; i0 < total; i0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < total) v[i] = __ldcg(reinterpret_cast<const float4 *>(g.o + static_cast<int64_t>(entry[warp][i0 + i].x) * g.hidden + n));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < total) {
+                const float f = __int_as_float(entry[warp][i0 + i].y);
+                y.x = fmaf(f, v[i].x, y.x), y.y = fmaf(f, v[i].y, y.y), y.z = fmaf(f, v[i].z, y.z), y.w = fmaf(f, v[i].w, y.w);
+            }
     }
     uint2 out;
     out.x = T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16;
@@ -504,7 +598,8 @@ int most_parts(int64_t units, int64_t kblocks) {
 
 struct MoeLayout {
     int parts_up, parts_down;
-    int64_t off_list, off_z, off_o, bytes;
+    bool gate_kernel;
+    int64_t off_list, off_z, off_o, off_h, bytes;
 };
 
 MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
@@ -515,29 +610,44 @@ MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t expe
     l.off_list = 0;
     l.off_z = up256((2 + 3 * experts + 4 * slots) * 4);
     l.off_o = l.off_z + up256(l.parts_up * slots * 2 * inner * 4);
-    l.bytes = l.off_o + up256(l.parts_down * slots * hidden * 4);
+    l.off_h = l.off_o + up256(l.parts_down * slots * hidden * 4);
+    l.gate_kernel = tokens > kFewTokens;
+    l.bytes = l.off_h + (l.gate_kernel ? up256(2 * slots * inner * 2) : 0);
     return l;
 }
 
 template <typename T>
-cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, int smem, cudaStream_t stream) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, bool gate_kernel, int smem, cudaStream_t stream) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(1);
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cfg.gridDim = dim3((g.tokens + 31) / 32);
     cfg.blockDim = dim3(1024);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cfg.gridDim.x;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, moe_route_kernel, g);
+    cfg.numAttrs = 1;
     cfg.gridDim = dim3(g.sms);
     cfg.blockDim = dim3(kMoeThreads);
     cfg.dynamicSmemBytes = smem;
     g.map = up;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, false>, g);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, UP>, g);
+    if (gate_kernel) {
+        cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(g.slots) * (g.inner / 8) + 255) / 256));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_gate_kernel<T>, g);
+    }
+    cfg.gridDim = dim3(g.sms);
+    cfg.blockDim = dim3(kMoeThreads);
+    cfg.dynamicSmemBytes = smem;
     g.map = down;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, true>, g);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, gate_kernel ? moe_product_kernel<T, DOWN> : moe_product_kernel<T, DOWN_INLINE>, g);
     cfg.gridDim = dim3((g.hidden + 511) / 512, g.tokens);
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = 0;
@@ -548,9 +658,9 @@ cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &dow
 }  // namespace
 
 int prepare_moe_kernels() {
-    const void *const kernels[] = {reinterpret_cast<const void *>(moe_product_kernel<Bf16, false>), reinterpret_cast<const void *>(moe_product_kernel<Bf16, true>),
-                                   reinterpret_cast<const void *>(moe_product_kernel<Fp16, false>), reinterpret_cast<const void *>(moe_product_kernel<Fp16, true>)};
-    for (const void *k : kernels) {
+    void (*const kernels[])(MoeArgs) = {moe_product_kernel<Bf16, UP>, moe_product_kernel<Bf16, DOWN_INLINE>, moe_product_kernel<Bf16, DOWN>,
+                                        moe_product_kernel<Fp16, UP>, moe_product_kernel<Fp16, DOWN_INLINE>, moe_product_kernel<Fp16, DOWN>};
+    for (const auto k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
     }
@@ -592,10 +702,12 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     CUtensorMap up, down;
     st = encode_operand_map(&up, dtype, W13, hidden, experts * 2 * inner, 64);
     if (st == B200_OK) st = encode_operand_map(&down, dtype, W2, inner, experts * hidden, 128);
-    if (st != B200_OK) return st;
     const MoeLayout l = moe_layout(tokens, hidden, inner, experts, top_k);
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     const int64_t slots = tokens * top_k;
+    g.h = reinterpret_cast<uint16_t *>(ws + l.off_h);
+    if (st == B200_OK && l.gate_kernel) st = encode_operand_map(&g.map_h, dtype, g.h, inner, 2 * slots, 16);
+    if (st != B200_OK) return st;
     int *const list = reinterpret_cast<int *>(ws + l.off_list);
     g.list.header = list;
     g.list.expert = list + 2;
@@ -626,7 +738,7 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     g.slot_cols = static_cast<int>((tokens + 15) / 16 * 16);
     g.tmem_cols = pow2_at_least(2 * g.slot_cols);
     const int lists = static_cast<int>(up256(slots * 2) + up256(experts * 12));
-    const int smem = tokens <= 16 ? 113 * 1024 : kSmemLimit;
+    const int smem = tokens <= kFewTokens ? 113 * 1024 : kSmemLimit;
     g.ring_bytes = (smem - 1024 - lists - 512) / 1024 * 1024;
     g.off_token = g.ring_bytes;
     g.off_expert = g.off_token + static_cast<int>(up256(slots * 2));
@@ -634,7 +746,7 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     g.off_misc = g.off_bars + (2 * kMoeStages + 4) * 8;
     g.idesc = umma_idesc(128, 0, dtype == B200_BF16);
     g.budget = wait_budget_cycles();
-    const cudaError_t e = dtype == B200_BF16 ? launch_moe<Bf16>(g, up, down, smem, static_cast<cudaStream_t>(stream))
-                                             : launch_moe<Fp16>(g, up, down, smem, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = dtype == B200_BF16 ? launch_moe<Bf16>(g, up, down, l.gate_kernel, smem, static_cast<cudaStream_t>(stream))
+                                             : launch_moe<Fp16>(g, up, down, l.gate_kernel, smem, static_cast<cudaStream_t>(stream));
     return e != cudaSuccess ? record_cuda_error(e) : B200_OK;
 }

@@ -48,6 +48,11 @@ __device__ __forceinline__ void mbar_arrive_many(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 
+// A bit set in a word of another CTA's shared memory (address from mapa_shared).
+__device__ __forceinline__ void red_or_cluster(uint32_t cluster_addr, uint32_t bits) {
+    asm volatile("red.shared::cluster.or.b32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
+}
+
 // 16 bytes global -> shared without passing through registers (L2 only); complete after cp_async_wait_all.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
