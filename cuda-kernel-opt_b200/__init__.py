@@ -257,49 +257,59 @@ def gemm(A, Bt, Cm=None, D=None, alpha=1.0, beta=0.0, params: Params | None = No
     return D
 
 
-def _require(ok, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+_CODES = {}   # torch dtype -> B200_F16 / B200_BF16, filled on first use
 
 
-def _check_operands(where: str, device, *named) -> None:
-    """named: (name, tensor, dtype, shape); a tensor of None passes."""
-    for name, t, dtype, shape in named:
-        if t is not None and not (t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous()):
-            raise ValueError(f"{where}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
-                             f"not {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
-
-
-class _On:
-    """Makes a tensor's device and the stream of the call current, so that what is allocated for the call (outputs, the
-    workspace) belongs to that stream. Does nothing where both are current already, the usual case."""
-
-    def __init__(self, device, stream):
+def _code(where: str, t) -> int:
+    if not _CODES:
         import torch
-        now = torch.cuda.current_stream(device)
-        self.stream = now.cuda_stream if stream is None else int(stream)
-        self.guard = None
-        if device.index != torch.cuda.current_device() or self.stream != now.cuda_stream:
-            on = now if self.stream == now.cuda_stream else torch.cuda.ExternalStream(self.stream, device) if self.stream else torch.cuda.default_stream(device)
-            self.guard = torch.cuda.stream(on)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        _CODES.update({torch.float16: F16, torch.bfloat16: BF16})
+    code = _CODES.get(t.dtype)
+    if code is None or not t.is_cuda:
+        raise ValueError(f"{where}: the operands must be fp16 or bf16 CUDA tensors, not {t.dtype} on {t.device}")
+    return code
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
+def _check(where: str, name: str, t, dtype, shape, device) -> None:
+    if not (t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous()):
+        raise ValueError(f"{where}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
+                         f"not {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
+
+
+def _on_stream(fn, args, device, stream):
+    """fn(*args, handle) with the tensors' device and the stream of the call current, so that what fn allocates (outputs, the
+    workspace) belongs to that stream's memory. Both usually are current already."""
+    import torch
+    raw = torch._C._cuda_getCurrentRawStream(device.index)
+    handle = raw if stream is None else int(stream)
+    if handle == raw and device.index == torch.cuda.current_device():
+        return fn(*args, handle)
+    on = torch.cuda.current_stream(device) if handle == raw else torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
+    with torch.cuda.stream(on):
+        return fn(*args, handle)
 
 
 def gemm_lora_workspace_bytes(M, N, K, num_adapters, rank) -> int:
     """b200_gemm_lora_workspace_bytes; -1 for sizes that the call refuses."""
     return lib().b200_gemm_lora_workspace_bytes(M, N, K, num_adapters, rank)
+
+
+def _gemm_lora(code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, sizes, stream):
+    import torch
+    M, N, K, S, R = sizes
+    L = lib()
+    if workspace is None:
+        need = L.b200_gemm_lora_workspace_bytes(M, N, K, S, R)
+        if need > 0:
+            workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=A.device)   # the quickest of torch's allocations
+    if D is None:
+        D = torch.empty_strided((M, N), (N, 1), dtype=A.dtype, device=A.device)
+    st = L.b200_gemm_lora(code, A.data_ptr(), Bt.data_ptr(), D.data_ptr(), M, N, K, lora_a.data_ptr(), lora_b.data_ptr(),
+                          lora_scale.data_ptr() if lora_scale is not None else None, row_adapter.data_ptr(), S, R,
+                          workspace.data_ptr() if workspace is not None else None, workspace.nbytes if workspace is not None else 0, stream)
+    if st != OK:
+        raise B200Error(st, "b200_gemm_lora")
+    return D
 
 
 def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, workspace=None, stream=None):
@@ -312,32 +322,45 @@ def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, works
     torch's current one); the operands must be ready there. Raises ValueError for tensors that do not fit together and
     B200Error for what the library refuses."""
     import torch
-    _require(A.is_cuda and A.dtype in (torch.float16, torch.bfloat16) and A.dim() == 2, "gemm_lora: A must be a 2-d fp16 or bf16 CUDA tensor")
-    _require(Bt.dim() == 2 and lora_a.dim() == 3, "gemm_lora: Bt must have 2 dimensions and lora_a 3")
-    M, K = A.shape
-    N = Bt.shape[0]
-    S, R = lora_a.shape[0], lora_a.shape[1]
-    dev, t = A.device, A.dtype
-    _check_operands("gemm_lora", dev, ("A", A, t, (M, K)), ("Bt", Bt, t, (N, K)), ("lora_a", lora_a, t, (S, R, K)), ("lora_b", lora_b, t, (S, N, R)),
-                    ("row_adapter", row_adapter, torch.int32, (M,)), ("lora_scale", lora_scale, torch.float32, (S,)), ("D", D, t, (M, N)))
-    L = lib()
-    with _On(dev, stream) as sptr:
-        need = L.b200_gemm_lora_workspace_bytes(M, N, K, S, R)
-        if workspace is None and need > 0:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        if D is None:
-            D = torch.empty((M, N), dtype=t, device=dev)
-        st = L.b200_gemm_lora(BF16 if t == torch.bfloat16 else F16, A.data_ptr(), Bt.data_ptr(), D.data_ptr(), M, N, K, lora_a.data_ptr(),
-                              lora_b.data_ptr(), _ptr(lora_scale), row_adapter.data_ptr(), S, R, _ptr(workspace),
-                              workspace.numel() * workspace.element_size() if workspace is not None else 0, sptr)
-    if st != OK:
-        raise B200Error(st, "b200_gemm_lora")
-    return D
+    code = _code("gemm_lora", A)
+    if A.dim() != 2 or Bt.dim() != 2 or lora_a.dim() != 3:
+        raise ValueError("gemm_lora: A and Bt must have 2 dimensions and lora_a 3")
+    (M, K), N, (S, R, _), dev, t, i32 = A.shape, Bt.shape[0], lora_a.shape, A.device, A.dtype, torch.int32
+    _check("gemm_lora", "A", A, t, (M, K), dev)
+    _check("gemm_lora", "Bt", Bt, t, (N, K), dev)
+    _check("gemm_lora", "lora_a", lora_a, t, (S, R, K), dev)
+    _check("gemm_lora", "lora_b", lora_b, t, (S, N, R), dev)
+    _check("gemm_lora", "row_adapter", row_adapter, i32, (M,), dev)
+    if lora_scale is not None:
+        _check("gemm_lora", "lora_scale", lora_scale, torch.float32, (S,), dev)
+    if D is not None:
+        _check("gemm_lora", "D", D, t, (M, N), dev)
+    return _on_stream(_gemm_lora, (code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, (M, N, K, S, R)), dev, stream)
 
 
 def moe_workspace_bytes(tokens, hidden, inner, experts, top_k) -> int:
     """b200_moe_workspace_bytes; -1 for sizes that the call refuses."""
     return lib().b200_moe_workspace_bytes(tokens, hidden, inner, experts, top_k)
+
+
+def _moe(code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, sizes, stream):
+    import torch
+    T, H, I, E, k = sizes
+    L = lib()
+    if workspace is None:
+        need = max(L.b200_moe_workspace_bytes(T, H, I, E, k), 0)
+        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=X.device)   # the quickest of torch's allocations
+    if Y is None:
+        Y = torch.empty_like(X)
+    if ids is None:
+        ids = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.int32, device=X.device)
+    if weights is None:
+        weights = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.float32, device=X.device)
+    st = L.b200_moe(code, X.data_ptr(), logits.data_ptr(), W13.data_ptr(), W2.data_ptr(), Y.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, H, I, E,
+                    k, 1 if normalise else 0, workspace.data_ptr(), workspace.nbytes, stream)
+    if st != OK:
+        raise B200Error(st, "b200_moe")
+    return Y, ids, weights
 
 
 def moe(X, logits, W13, W2, top_k, normalise=True, Y=None, ids=None, weights=None, workspace=None, stream=None):
@@ -349,33 +372,21 @@ def moe(X, logits, W13, W2, top_k, normalise=True, Y=None, ids=None, weights=Non
     logits. Outputs and the workspace are allocated, on the stream of the call, when not given; stream as in gemm_lora.
     Raises ValueError for tensors that do not fit together and B200Error for what the library refuses."""
     import torch
-    _require(X.is_cuda and X.dtype in (torch.float16, torch.bfloat16) and X.dim() == 2, "moe: X must be a 2-d fp16 or bf16 CUDA tensor")
-    _require(W2.dim() == 3, "moe: W2 must have 3 dimensions")
-    T, H = X.shape
-    E, I = W2.shape[0], W2.shape[2]
-    dev, t = X.device, X.dtype
-    _check_operands("moe", dev, ("X", X, t, (T, H)), ("logits", logits, torch.float32, (T, E)), ("W13", W13, t, (E, 2 * I, H)), ("W2", W2, t, (E, H, I)),
-                    ("Y", Y, t, (T, H)), ("ids", ids, torch.int32, (T, top_k)), ("weights", weights, torch.float32, (T, top_k)))
-    L = lib()
-    with _On(dev, stream) as sptr:
-        need = L.b200_moe_workspace_bytes(T, H, I, E, top_k)
-        if need < 0:      # refused; the call says why
-            st = L.b200_moe(BF16 if t == torch.bfloat16 else F16, None, None, None, None, None, None, None, T, H, I, E, top_k, int(normalise), None, 0, sptr)
-            raise B200Error(st, "b200_moe")
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        if Y is None:
-            Y = torch.empty((T, H), dtype=t, device=dev)
-        if ids is None:
-            ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-        if weights is None:
-            weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-        st = L.b200_moe(BF16 if t == torch.bfloat16 else F16, X.data_ptr(), logits.data_ptr(), W13.data_ptr(), W2.data_ptr(), Y.data_ptr(),
-                        ids.data_ptr(), weights.data_ptr(), T, H, I, E, top_k, int(normalise), workspace.data_ptr(),
-                        workspace.numel() * workspace.element_size(), sptr)
-    if st != OK:
-        raise B200Error(st, "b200_moe")
-    return Y, ids, weights
+    code = _code("moe", X)
+    if X.dim() != 2 or W2.dim() != 3:
+        raise ValueError("moe: X must have 2 dimensions and W2 3")
+    (T, H), (E, _, I), dev, t, f32 = X.shape, W2.shape, X.device, X.dtype, torch.float32
+    _check("moe", "X", X, t, (T, H), dev)
+    _check("moe", "logits", logits, f32, (T, E), dev)
+    _check("moe", "W13", W13, t, (E, 2 * I, H), dev)
+    _check("moe", "W2", W2, t, (E, H, I), dev)
+    if Y is not None:
+        _check("moe", "Y", Y, t, (T, H), dev)
+    if ids is not None:
+        _check("moe", "ids", ids, torch.int32, (T, top_k), dev)
+    if weights is not None:
+        _check("moe", "weights", weights, f32, (T, top_k), dev)
+    return _on_stream(_moe, (code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, (T, H, I, E, top_k)), dev, stream)
 
 
 def device_status(stream=None):

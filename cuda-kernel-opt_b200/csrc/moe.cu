@@ -37,7 +37,10 @@ constexpr int kMoeStages = 16;      // most stages of the ring
 constexpr int kMoeLoaders = 8;      // warps that bring the activations of a K block
 constexpr int kMoeThreads = (2 + 4 + kMoeLoaders) * 32;
 constexpr int kMaxParts = 16;
-constexpr int kFewTokens = 16;      // up to here the loader warps of DOWN compute the gated values, beyond a kernel does
+constexpr int kMaxHidden = 65536;
+constexpr int kTileWords = kMaxHidden / 128 / 32;   // a bit per tile of Y
+constexpr int kFewSlots = 128;      // (token, choice) pairs and tokens up to which two kernels do all of it; the tokens also
+constexpr int kFewTokens = 64;      // bound a stage of the smaller ring, which must hold two
 constexpr int kGridSms = 148;       // what the workspace is sized for; another count only changes how tiles are cut
 constexpr int kBoxBytes = 16 * 128;      // 16 slots of 64 gated values
 constexpr int kWeightBytes = 128 * 128;  // one K block of a weight tile: 128 rows of 64 elements
@@ -69,9 +72,10 @@ struct alignas(64) MoeArgs {
     int tokens, hidden, inner, experts, top_k, normalise, slots;
     int parts_up, parts_down;
     int sms;
-    int ring_bytes, off_token, off_expert, off_bars, off_misc;
+    int ring_bytes, off_slots, off_experts, off_bars, off_misc;
     int tmem_cols, slot_cols;
     uint32_t idesc;           // with N = 0
+    int *arrived;             // few: per tile of Y, the warps that are done with it
     int *status;
     long long budget;
 };
@@ -130,43 +134,87 @@ __device__ __forceinline__ void choose_experts(const float *logits, int experts,
     for (int j = 0; j < top_k; ++j) {
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
         if (most == 0u) break;
-        const uint32_t e = __reduce_min_sync(0xffffffffu, best == most ? static_cast<uint32_t>(lane + 32 * best_i) : 0xffffffffu);
-        if (lane == static_cast<int>(e & 31u)) {
+        int e = lane + 32 * best_i, winner = best == most;
+        const uint32_t equal = __ballot_sync(0xffffffffu, winner);
+        int from = __ffs(equal) - 1;
+        if (equal & (equal - 1u)) {   // several lanes: the lowest index wins
+            const int low = static_cast<int>(__reduce_min_sync(0xffffffffu, winner ? static_cast<uint32_t>(e) : 0xffffffffu));
+            from = low & 31;
+            winner = lane == from;
+        }
+        e = __shfl_sync(0xffffffffu, e, from);
+        if (lane == j) id = e, chosen = most;
+        if (winner) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (i == best_i) key[i] = 0u;
             look();
         }
-        if (lane == j) id = static_cast<int>(e), chosen = most;
+        __syncwarp();
     }
     weight = id >= 0 ? expf(key_logit(chosen) - top) : 0.0f;
     if (normalise) sum = warp_sum(weight);
     if (id >= 0) weight /= sum;
 }
 
+__device__ __forceinline__ void choose(const MoeArgs &g, int t, int lane, int &id, float &weight) {
+    const float *const row = g.logits + static_cast<int64_t>(t) * g.experts;
+    if (g.experts <= 32) choose_experts<1>(row, g.experts, g.top_k, g.normalise, lane, id, weight);
+    else if (g.experts <= 64) choose_experts<2>(row, g.experts, g.top_k, g.normalise, lane, id, weight);
+    else if (g.experts <= 128) choose_experts<4>(row, g.experts, g.top_k, g.normalise, lane, id, weight);
+    else if (g.experts <= 256) choose_experts<8>(row, g.experts, g.top_k, g.normalise, lane, id, weight);
+    else choose_experts<16>(row, g.experts, g.top_k, g.normalise, lane, id, weight);
+}
+
+// One warp: emit(position among the chosen, expert, tokens, first slot) for every expert that a token chose, in ascending order;
+// mask[e * words ..] holds the tokens of expert e as bits. Returns how many are chosen and the most tokens of one.
+template <typename Emit>
+__device__ __forceinline__ int2 list_experts(const uint32_t *mask, int words, int experts, int lane, Emit emit) {
+    int chosen = 0, slots = 0, most = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+        const int e = e0 + lane;
+        int n = 0;
+        if (e < experts)
+            for (int i = 0; i < words; ++i) n += __popc(mask[e * words + i]);
+        const uint32_t ballot = __ballot_sync(0xffffffffu, n > 0);
+        if (ballot == 0u) continue;
+        int before = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        if (n > 0) emit(chosen + __popc(ballot & ((1u << lane) - 1u)), e, n, slots + before - n);
+        chosen += __popc(ballot);
+        slots += __shfl_sync(0xffffffffu, before, 31);
+        most = max(most, static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(n))));
+    }
+    return make_int2(chosen, most);
+}
+
+// The place of token t among the tokens of its expert.
+__device__ __forceinline__ int rank_of(const uint32_t *mask, int words, int e, int t) {
+    int r = __popc(mask[e * words + (t >> 5)] & ((1u << (t & 31)) - 1u));
+    for (int i = 0; i < (t >> 5); ++i) r += __popc(mask[e * words + i]);
+    return r;
+}
+
 // One cluster of up to eight blocks, a warp per token; its first block then lists the chosen experts and their tokens.
 __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__ MoeArgs g) {
-    __shared__ uint32_t mask[B200_MOE_MAX_EXPERTS][B200_MOE_MAX_TOKENS / 32];   // the tokens of an expert (of the first block)
-    __shared__ short place[B200_MOE_MAX_EXPERTS];                               // its position among the chosen
-    __shared__ int first[B200_MOE_MAX_EXPERTS];                                 // its first slot
+    __shared__ uint32_t mask[B200_MOE_MAX_EXPERTS * (B200_MOE_MAX_TOKENS / 32)];   // the tokens of an expert (of the first block)
+    __shared__ short place[B200_MOE_MAX_EXPERTS];                                  // its position among the chosen
+    __shared__ int first[B200_MOE_MAX_EXPERTS];                                    // its first slot
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int words = (g.tokens + 31) / 32;
     if (blockIdx.x == 0)
-        for (int i = tid; i < g.experts * words; i += 1024) mask[i / words][i % words] = 0u;
+        for (int i = tid; i < g.experts * words; i += 1024) mask[i] = 0u;
     cluster_arrive();
     griddep_wait();
     griddep_launch_dependents();
     const int t = blockIdx.x * 32 + warp;
     int id = -1;
     float w = 0.0f;
-    if (t < g.tokens) {
-        const float *const row = g.logits + static_cast<int64_t>(t) * g.experts;
-        if (g.experts <= 32) choose_experts<1>(row, g.experts, g.top_k, g.normalise, lane, id, w);
-        else if (g.experts <= 64) choose_experts<2>(row, g.experts, g.top_k, g.normalise, lane, id, w);
-        else if (g.experts <= 128) choose_experts<4>(row, g.experts, g.top_k, g.normalise, lane, id, w);
-        else if (g.experts <= 256) choose_experts<8>(row, g.experts, g.top_k, g.normalise, lane, id, w);
-        else choose_experts<16>(row, g.experts, g.top_k, g.normalise, lane, id, w);
-    }
+    if (t < g.tokens) choose(g, t, lane, id, w);
     cluster_wait();                                         // the first block's masks are zero
     if (t < g.tokens && lane < g.top_k) {
         const int at = t * g.top_k + lane;
@@ -174,48 +222,29 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__
         g.list.weight[at] = w;
         if (g.ids_out) g.ids_out[at] = id;
         if (g.weights_out) g.weights_out[at] = w;
-        if (id >= 0) red_or_cluster(mapa_shared(smem_u32(&mask[id][t >> 5]), 0), 1u << (t & 31));
+        if (id >= 0) red_or_cluster(mapa_shared(smem_u32(&mask[id * words + (t >> 5)]), 0), 1u << (t & 31));
     }
     cluster_arrive();
     cluster_wait();
     if (blockIdx.x != 0) return;
     if (warp == 0) {
-        int chosen = 0, slots = 0, most = 0;
-        for (int e0 = 0; e0 < g.experts; e0 += 32) {
-            const int e = e0 + lane;
-            int n = 0;
-            if (e < g.experts)
-                for (int i = 0; i < words; ++i) n += __popc(mask[e][i]);
-            const uint32_t ballot = __ballot_sync(0xffffffffu, n > 0);
-            int before = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += v;
-            }
-            if (n > 0) {
-                const int at = chosen + __popc(ballot & ((1u << lane) - 1u));
-                g.list.expert[at] = e;
-                g.list.count[at] = n;
-                g.list.base[at] = slots + before - n;
-                place[e] = static_cast<short>(at);
-                first[e] = slots + before - n;
-            }
-            chosen += __popc(ballot);
-            slots += __shfl_sync(0xffffffffu, before, 31);
-            most = max(most, static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(n))));
-        }
+        const int2 n = list_experts(mask, words, g.experts, lane, [&](int at, int e, int count, int base) {
+            g.list.expert[at] = e;
+            g.list.count[at] = count;
+            g.list.base[at] = base;
+            place[e] = static_cast<short>(at);
+            first[e] = base;
+        });
         if (lane == 0) {
-            g.list.header[0] = chosen;
-            g.list.header[1] = most;
+            g.list.header[0] = n.x;
+            g.list.header[1] = n.y;
         }
     }
     __syncthreads();
     for (int at = tid; at < g.slots; at += 1024) {
         const int t = at / g.top_k, e = __ldcg(g.list.slot + at);
         if (e < 0) continue;
-        int slot = first[e] + __popc(mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
-        for (int i = 0; i < (t >> 5); ++i) slot += __popc(mask[e][i]);
+        const int slot = first[e] + rank_of(mask, words, e, t);
         g.list.token[slot] = t;
         g.list.slot[at] = slot;
         g.list.active[at] = place[e];
@@ -227,18 +256,25 @@ struct Segment {
     int ai, tile, kb0, kb1, part;
 };
 
+// Tiles in a row are those of one expert, or with BY_TILE the experts of one tile.
+template <bool BY_TILE>
 struct Walker {
-    int q, end, tiles, cta;
+    int q, end, tiles, chosen, cta;
     Cut cut;
-    __device__ __forceinline__ Walker(const Cut &c, int tiles_, int cta_) : tiles(tiles_), cta(cta_), cut(c) {
+    __device__ __forceinline__ Walker(const Cut &c, int tiles_, int chosen_, int cta_) : tiles(tiles_), chosen(chosen_), cta(cta_), cut(c) {
         q = min(static_cast<long long>(cta) * c.len, static_cast<long long>(c.total));
         end = min(q + c.len, c.total);
     }
     __device__ __forceinline__ bool next(Segment &s) {
         if (q >= end) return false;
         const int unit = q / cut.kblocks;
-        s.ai = unit / tiles;
-        s.tile = unit - s.ai * tiles;
+        if (BY_TILE) {
+            s.tile = unit / chosen;
+            s.ai = unit - s.tile * chosen;
+        } else {
+            s.ai = unit / tiles;
+            s.tile = unit - s.ai * tiles;
+        }
         s.kb0 = q - unit * cut.kblocks;
         s.kb1 = min(cut.kblocks, s.kb0 + end - q);
         s.part = cta - cut.first_cta(unit);
@@ -248,43 +284,96 @@ struct Walker {
 };
 
 enum Product {
-    UP,           // gate and up rows times the tokens of X, gathered by the loader warps
-    DOWN_INLINE,  // W2 times the gated values, which the loader warps compute from UP's parts
-    DOWN          // W2 times the gated values that moe_gate_kernel has left in the workspace, by TMA
+    UP,        // gate and up rows times the tokens of X, gathered by the loader warps
+    DOWN,      // W2 times the gated values that moe_gate_kernel has left in the workspace, by TMA
+    UP_FEW,    // UP where every CTA makes the router's choice for itself
+    DOWN_FEW   // so does this one; its loader warps compute the gated values from UP's parts, and the last CTA to finish a tile
+               // of Y adds the tile's parts
 };
 
-// The gated value of eight neighbouring inner rows of one slot from UP's parts (ascending), as pairs of 16-bit numbers.
-// The exponential and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th of an fp16.
+// The gated value of four neighbouring inner rows of one slot from UP's parts (ascending, four of them in flight), as pairs of
+// 16-bit numbers. The exponential and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th
+// of an fp16.
 template <typename T>
-__device__ __forceinline__ void gated_values(const float *z, int inner, int parts, int64_t part_pitch, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    float gate[8] = {}, up[8] = {};
-    for (int p = 0; p < parts; ++p, z += part_pitch) {
-        const float4 a = __ldcg(reinterpret_cast<const float4 *>(z)), b = __ldcg(reinterpret_cast<const float4 *>(z + 4));
-        const float4 c = __ldcg(reinterpret_cast<const float4 *>(z + inner)), d = __ldcg(reinterpret_cast<const float4 *>(z + inner + 4));
-        gate[0] += a.x, gate[1] += a.y, gate[2] += a.z, gate[3] += a.w, gate[4] += b.x, gate[5] += b.y, gate[6] += b.z, gate[7] += b.w;
-        up[0] += c.x, up[1] += c.y, up[2] += c.z, up[3] += c.w, up[4] += d.x, up[5] += d.y, up[6] += d.z, up[7] += d.w;
-    }
+__device__ __forceinline__ void gated_values(const float *z, int inner, int parts, int64_t part_pitch, uint2 &hi, uint2 &lo) {
+    float4 gate = make_float4(0.0f, 0.0f, 0.0f, 0.0f), up = gate;
+    for (int p0 = 0; p0 < parts; p0 += 4, z += 4 * part_pitch) {
+        float4 a[4], b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint16_t h0, h1, l0, l1;
-        T::split(__fdividef(gate[2 * i], 1.0f + __expf(-gate[2 * i])) * up[2 * i], h0, l0);
-        T::split(__fdividef(gate[2 * i + 1], 1.0f + __expf(-gate[2 * i + 1])) * up[2 * i + 1], h1, l1);
-        hi[i] = h0 | static_cast<uint32_t>(h1) << 16;
-        lo[i] = l0 | static_cast<uint32_t>(l1) << 16;
+        for (int p = 0; p < 4; ++p)
+            if (p0 + p < parts) {
+                a[p] = __ldcg(reinterpret_cast<const float4 *>(z + p * part_pitch));
+                b[p] = __ldcg(reinterpret_cast<const float4 *>(z + p * part_pitch + inner));
+            }
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            if (p0 + p < parts) {
+                gate.x += a[p].x, gate.y += a[p].y, gate.z += a[p].z, gate.w += a[p].w;
+                up.x += b[p].x, up.y += b[p].y, up.z += b[p].z, up.w += b[p].w;
+            }
     }
+    const float g[4] = {gate.x, gate.y, gate.z, gate.w}, u[4] = {up.x, up.y, up.z, up.w};
+    uint16_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) T::split(__fdividef(g[i], 1.0f + __expf(-g[i])) * u[i], h[i], l[i]);
+    hi = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+    lo = make_uint2(l[0] | static_cast<uint32_t>(l[1]) << 16, l[2] | static_cast<uint32_t>(l[3]) << 16);
+}
+
+// One warp, 128 columns of one token, four per lane from n on: the weighted parts, in ascending order within a choice, choices in
+// descending order of their logits. Lane j < top_k brings choice j: its slot, the number of its parts in these
+// columns, its weight. The warp first lists where the parts are, so that four loads are in flight at a time; eight, and
+// with them a longer stretch of code that runs once per launch and has to be fetched for that, measured slower
+// (one token, 8 of 128 experts of 2048 x 768: 28.7 against 34.4 us for the layer).
+template <typename T>
+__device__ __forceinline__ void combine(const MoeArgs &g, int2 *entry, int t, int n, int lane, int slot, int parts, float w) {
+    constexpr int kBatch = 4;
+    int before = parts;
+#pragma unroll 1
+    for (int o = 1; o < B200_MOE_MAX_TOP_K; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, B200_MOE_MAX_TOP_K - 1);
+    __syncwarp();
+    for (int p = 0; p < parts; ++p) entry[before - parts + p] = make_int2(p * g.slots + slot, __float_as_int(w));
+    __syncwarp();
+    if (n >= g.hidden) return;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < total; i0 += kBatch) {
+        float4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (i0 + i < total) v[i] = __ldcg(reinterpret_cast<const float4 *>(g.o + static_cast<int64_t>(entry[i0 + i].x) * g.hidden + n));
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (i0 + i < total) {
+                const float f = __int_as_float(entry[i0 + i].y);
+                y.x = fmaf(f, v[i].x, y.x), y.y = fmaf(f, v[i].y, y.y), y.z = fmaf(f, v[i].z, y.z), y.w = fmaf(f, v[i].w, y.w);
+            }
+    }
+    *reinterpret_cast<uint2 *>(g.Y + static_cast<int64_t>(t) * g.hidden + n) =
+        make_uint2(T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16, T::round(y.z) | static_cast<uint32_t>(T::round(y.w)) << 16);
 }
 
 template <typename T, Product P>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __grid_constant__ MoeArgs g) {
+    constexpr bool kUp = P == UP || P == UP_FEW, kFew = P == UP_FEW || P == DOWN_FEW;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t *const sm = smem_raw + (ring - raw);
-    uint16_t *const token_s = reinterpret_cast<uint16_t *>(sm + g.off_token);
-    int *const expert_s = reinterpret_cast<int *>(sm + g.off_expert);
+    float *const weight_s = reinterpret_cast<float *>(sm + g.off_slots);                    // few: per (token, choice)
+    uint16_t *const token_s = reinterpret_cast<uint16_t *>(weight_s + (kFew ? g.slots : 0));   // per slot
+    int16_t *const slot_s = reinterpret_cast<int16_t *>(token_s + g.slots);                 // few: per (token, choice), -1 without an expert
+    int16_t *const active_s = slot_s + g.slots;                                             // few: per (token, choice)
+    int *const expert_s = reinterpret_cast<int *>(sm + g.off_experts);
     int *const count_s = expert_s + g.experts, *const base_s = count_s + g.experts;
+    uint32_t *const mask_s = reinterpret_cast<uint32_t *>(base_s + g.experts);              // few
+    const int words = (g.tokens + 31) / 32;
+    int16_t *const place_s = reinterpret_cast<int16_t *>(mask_s + g.experts * words);       // few
     const uint32_t full0 = ring + g.off_bars, empty0 = full0 + 8 * kMoeStages, acc_full0 = empty0 + 8 * kMoeStages, acc_empty0 = acc_full0 + 16;
-    volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // [0] abort flag, [1] tensor-memory base
+    volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // abort flag, tensor-memory base, chosen experts, most tokens; few: tiles to add
     const WaitCtx wait = {g.status, misc, g.budget};
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -295,6 +384,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0;
+    if (P == DOWN_FEW && tid >= 64 && tid < 64 + kTileWords) misc[4 + tid - 64] = 0;
+    if (kFew)
+        for (int i = tid; i < g.experts * words; i += kMoeThreads) mask_s[i] = 0u;
     if (tid == 32) tma_prefetch_desc(&g.map);
     if (P == DOWN && tid == 64) tma_prefetch_desc(&g.map_h);
     if (warp == 1) {
@@ -304,28 +396,92 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    // UP waits for the route kernel; every CTA of UP says so before DOWN may start, so DOWN finds the lists (and all that came
-    // before the call) complete without a wait of its own, and waits later for UP's sums.
-    if (P == UP) griddep_wait();
+    // UP waits for what came before (the route kernel, or with few tokens all work before the call); every CTA of UP says so
+    // before DOWN may start, so DOWN finds lists, logits and weights complete without a wait of its own, and waits later for
+    // UP's sums.
+    if (kUp) griddep_wait();
     griddep_launch_dependents();
-    const int chosen = __ldcg(g.list.header), most = __ldcg(g.list.header + 1);
-    for (int i = tid; i < chosen; i += kMoeThreads) {
-        expert_s[i] = __ldcg(g.list.expert + i);
-        count_s[i] = __ldcg(g.list.count + i);
-        base_s[i] = __ldcg(g.list.base + i);
+    if (kUp && kFew && blockIdx.x == 0)
+        for (int i = tid; i < (g.hidden + 127) / 128; i += kMoeThreads) g.arrived[i] = 0;
+    if (kFew && g.tokens == 1) {
+        // one token: its choices are the list
+        if (warp == 0) {
+            int id;
+            float w;
+            choose(g, 0, lane, id, w);
+            const int n = __popc(__ballot_sync(0xffffffffu, id >= 0));
+            if (lane < g.top_k) {
+                expert_s[lane] = id;
+                count_s[lane] = 1;
+                base_s[lane] = lane;
+                token_s[lane] = 0;
+                slot_s[lane] = static_cast<int16_t>(id >= 0 ? lane : -1);
+                active_s[lane] = static_cast<int16_t>(lane);
+                weight_s[lane] = w;
+                if (kUp && blockIdx.x == 0) {
+                    if (g.ids_out) g.ids_out[lane] = id;
+                    if (g.weights_out) g.weights_out[lane] = w;
+                }
+            }
+            if (lane == 0) misc[2] = n, misc[3] = n > 0;
+        }
+    } else if (kFew) {
+        for (int t = warp; t < g.tokens; t += kMoeThreads / 32) {
+            int id;
+            float w;
+            choose(g, t, lane, id, w);
+            if (lane < g.top_k) {
+                const int at = t * g.top_k + lane;
+                slot_s[at] = static_cast<int16_t>(id);         // the expert for now
+                weight_s[at] = w;
+                if (id >= 0) atomicOr(&mask_s[id * words + (t >> 5)], 1u << (t & 31));
+                if (kUp && blockIdx.x == 0) {
+                    if (g.ids_out) g.ids_out[at] = id;
+                    if (g.weights_out) g.weights_out[at] = w;
+                }
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const int2 n = list_experts(mask_s, words, g.experts, lane, [&](int at, int e, int count, int base) {
+                expert_s[at] = e;
+                count_s[at] = count;
+                base_s[at] = base;
+                place_s[e] = static_cast<int16_t>(at);
+            });
+            if (lane == 0) misc[2] = n.x, misc[3] = n.y;
+        }
+        __syncthreads();
+        for (int at = tid; at < g.slots; at += kMoeThreads) {
+            const int t = at / g.top_k, e = slot_s[at];
+            if (e < 0) continue;
+            const int slot = base_s[place_s[e]] + rank_of(mask_s, words, e, t);
+            token_s[slot] = static_cast<uint16_t>(t);
+            slot_s[at] = static_cast<int16_t>(slot);
+            active_s[at] = place_s[e];
+        }
+    } else {
+        const int n = __ldcg(g.list.header);
+        if (tid == 0) misc[2] = n, misc[3] = __ldcg(g.list.header + 1);
+        for (int i = tid; i < n; i += kMoeThreads) {
+            expert_s[i] = __ldcg(g.list.expert + i);
+            count_s[i] = __ldcg(g.list.count + i);
+            base_s[i] = __ldcg(g.list.base + i);
+        }
+        if (kUp)
+            for (int i = tid; i < g.slots; i += kMoeThreads) token_s[i] = static_cast<uint16_t>(__ldcg(g.list.token + i));
     }
-    if (P == UP)
-        for (int i = tid; i < g.slots; i += kMoeThreads) token_s[i] = static_cast<uint16_t>(__ldcg(g.list.token + i));
     __syncthreads();
+    const int chosen = __shfl_sync(0xffffffffu, misc[2], 0), most = __shfl_sync(0xffffffffu, misc[3], 0);
     const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[1]), 0);
 
     const int tiles_up = (g.inner + 63) / 64, kb_up = (g.hidden + 63) / 64;
-    const int tiles = P != UP ? (g.hidden + 127) / 128 : tiles_up;
-    const Cut cut(chosen * tiles, P != UP ? tiles_up : kb_up, g.sms, P != UP ? g.parts_down : g.parts_up);
+    const int tiles = !kUp ? (g.hidden + 127) / 128 : tiles_up;
+    const Cut cut(chosen * tiles, !kUp ? tiles_up : kb_up, g.sms, !kUp ? g.parts_down : g.parts_up);
     const uint32_t rows_bytes = static_cast<uint32_t>((most + 15) / 16 * 16 * 128);   // the activations of a K block (16-bit values)
-    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (P != UP ? 2 : 1);
+    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (!kUp ? 2 : 1);
     const int stages = min(kMoeStages, static_cast<int>(g.ring_bytes / stage_bytes));
-    Walker walk(cut, tiles, blockIdx.x);
+    Walker<P == DOWN_FEW> walk(cut, tiles, chosen, blockIdx.x);
     Segment s;
     int st = 0;
     uint32_t ph = 0;
@@ -335,7 +491,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         const bool issuer = elect_one();
         const uint64_t once = l2_policy(1);
         bool ok = true;
-        Walker ahead = walk;
+        Walker<P == DOWN_FEW> ahead = walk;
         Segment f;
         int fst = 0, fkb = 0, filled = 0;
         if (P == DOWN) {
@@ -353,7 +509,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         while (ok && walk.next(s)) {
             const int e = expert_s[s.ai];
             const int boxes = (count_s[s.ai] + 15) / 16;
-            const int row = P != UP ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
+            const int row = !kUp ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
                 if (P == DOWN && filled > 0) {
                     --filled;                              // its weights are on their way
@@ -364,7 +520,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                         const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
                         mbar_arrive_expect_tx(bar, kWeightBytes + (P == DOWN ? boxes * 2 * kBoxBytes : 0));
                         tma_load_2d_hint(dst, &g.map, bar, kb * 64, row, once);
-                        if (P == UP) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
+                        if (kUp) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
                     }
                 }
                 if (P == DOWN && issuer) {
@@ -398,7 +554,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         umma_f16<1>(d, a + 2 * i, b + 2 * i, idesc, kb > s.kb0 || i > 0);
-                        if (P != UP) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
+                        if (!kUp) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
                     }
                     umma_commit<1>(empty0 + 8 * st);
                 }
@@ -412,14 +568,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         const int quarter = warp & 3;
         const int r = quarter * 32 + lane;                 // row of the tile
         bool ok = true;
-        if (P != UP) griddep_wait();                          // in every CTA, with work or without: DOWN must not complete before UP
+        if (!kUp) griddep_wait();                          // in every CTA, with work or without: DOWN must not complete before UP
         for (int n = 0; ok && walk.next(s); ++n) {
             const int acc = n & 1, count = count_s[s.ai];
             const int64_t slot = static_cast<int64_t>(s.part) * g.slots + base_s[s.ai];
             float *out;
             int pitch;
             bool mine;
-            if (P != UP) {
+            if (!kUp) {
                 mine = s.tile * 128 + r < g.hidden;
                 pitch = g.hidden;
                 out = g.o + slot * pitch + s.tile * 128 + r;
@@ -446,7 +602,23 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty0 + 8 * acc);
+            if constexpr (P == DOWN_FEW) {
+                // With the last of its experts this CTA is done with the tile. Four warps of each of its CTAs count; the CTA
+                // whose warp is the last one adds the parts, when its own stretch is done.
+                auto rest = walk;
+                Segment after;
+                if (rest.next(after) && after.tile == s.tile) continue;
+                const int q0 = s.tile * chosen * cut.kblocks, ctas = (q0 + chosen * cut.kblocks - 1) / cut.len - q0 / cut.len + 1;
+                __threadfence();
+                __syncwarp();
+                if (lane == 0 && atomicAdd(g.arrived + s.tile, 1) == 4 * ctas - 1) {
+                    __threadfence();
+                    atomicOr(const_cast<int *>(misc) + 4 + (s.tile >> 5), 1 << (s.tile & 31));
+                }
+            }
         }
+        if (P == DOWN_FEW && chosen == 0)
+            for (int i = blockIdx.x * 128 + r; i < g.tokens * g.hidden; i += gridDim.x * 128) g.Y[i] = 0;
     } else if (P != DOWN) {
         // -------------------------------------------------------------- activations
         // The loader warps form groups that take the K blocks in turn, so that the latency of a block's loads is spread over
@@ -454,12 +626,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         // mistaken for the one two before it as long as there are no more groups than stages.
         const int group_warps = stages >= 8 ? 1 : stages >= 4 ? 2 : 4, groups = kMoeLoaders / group_warps;
         const int mine = (warp - 6) / group_warps, chunk = lane & 7;
-        const int row0 = (warp - 6) % group_warps * 4 + (lane >> 3), row_step = 4 * group_warps;
+        constexpr int kRows = kUp ? 4 : 2;              // rows that a warp takes at a time
+        const int row0 = (warp - 6) % group_warps * kRows + lane / (32 / kRows), row_step = kRows * group_warps;
         const Cut up(chosen * tiles_up, kb_up, g.sms, g.parts_up);
         const int64_t part_pitch = static_cast<int64_t>(g.slots) * 2 * g.inner;
         int turn = 0;
         bool ok = true;
-        if (P != UP) griddep_wait();
+        if (!kUp) griddep_wait();
         while (ok && walk.next(s)) {
             const int count = count_s[s.ai], base = base_s[s.ai];
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
@@ -468,19 +641,21 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                     if (!ok) break;
                     const uint32_t dst = ring + st * stage_bytes + kWeightBytes;
                     const int k = kb * 64 + chunk * 8;
-                    if (P == UP) {
+                    if (kUp) {
                         for (int r = row0; r < count; r += row_step) {
                             if (k < g.hidden) cp_async_16(dst + swizzled(r, chunk), g.X + static_cast<int64_t>(token_s[base + r]) * g.hidden + k);
                             else st_shared_v4(dst + swizzled(r, chunk), make_uint4(0, 0, 0, 0));
                         }
                         cp_async_wait_all();
                     } else {
-                        const int unit = s.ai * tiles_up + kb, parts = up.num_parts(unit);
+                        // sixteen lanes to a row, four values each: half a 16-byte chunk of the swizzled row
+                        const int parts = up.num_parts(s.ai * tiles_up + kb), k4 = kb * 64 + (lane & 15) * 4;
                         for (int r = row0; r < count; r += row_step) {
-                            uint32_t hi[4] = {}, lo[4] = {};
-                            if (k < g.inner) gated_values<T>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k, g.inner, parts, part_pitch, hi, lo);
-                            st_shared_v4(dst + swizzled(r, chunk), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                            st_shared_v4(dst + rows_bytes + swizzled(r, chunk), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                            uint2 hi = make_uint2(0, 0), lo = hi;
+                            if (k4 < g.inner) gated_values<T>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k4, g.inner, parts, part_pitch, hi, lo);
+                            const uint32_t at = dst + swizzled(r, (lane & 15) >> 1) + (lane & 1) * 8;
+                            st_shared_v2(at, hi);
+                            st_shared_v2(at + rows_bytes, lo);
                         }
                     }
                     fence_proxy_async_smem();
@@ -495,6 +670,23 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
 
     tc_fence_before_sync();
     __syncthreads();
+    if (P == DOWN_FEW && !misc[0]) {
+        // the ring is free now: each warp lists parts in its own corner of it
+        int2 *const entry = reinterpret_cast<int2 *>(sm) + warp * (B200_MOE_MAX_TOP_K * kMaxParts);
+        for (int tile = 0; tile < tiles; ++tile) {
+            if (!(misc[4 + (tile >> 5)] >> (tile & 31) & 1)) continue;
+            for (int t = warp; t < g.tokens; t += kMoeThreads / 32) {
+                int slot = -1, parts = 0;
+                float w = 0.0f;
+                if (lane < g.top_k) {
+                    slot = slot_s[t * g.top_k + lane];
+                    w = weight_s[t * g.top_k + lane];
+                    if (slot >= 0) parts = cut.num_parts(tile * chosen + active_s[t * g.top_k + lane]);
+                }
+                combine<T>(g, entry, t, tile * 128 + lane * 4, lane, slot, parts, w);
+            }
+        }
+    }
     if (warp == 1) {
         if (misc[0]) {   // aborted: give copies and MMAs in flight a bounded time to land before the memory goes
             const long long t0 = clock64();
@@ -506,13 +698,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     }
 }
 
-// The gated values for DOWN: eight inner rows of one slot per thread.
+// The gated values for DOWN: four inner rows of one slot per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
     griddep_launch_dependents();   // DOWN reads nothing of this kernel before its own wait
     griddep_wait();
-    const int chunks = g.inner / 8, tiles = (g.inner + 63) / 64;
-    const int at = blockIdx.x * 256 + threadIdx.x, slot = at / chunks, k = (at - slot * chunks) * 8;
+    const int chunks = g.inner / 4, tiles = (g.inner + 63) / 64;
+    const int at = blockIdx.x * 256 + threadIdx.x, slot = at / chunks, k = (at - slot * chunks) * 4;
     const int chosen = __ldcg(g.list.header);
     if (slot >= g.slots || chosen == 0) return;
     // the expert of a slot: the last one whose first slot is not behind it
@@ -524,21 +716,18 @@ __global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ M
     }
     if (slot >= __ldcg(g.list.base + lo_ai) + __ldcg(g.list.count + lo_ai)) return;
     const Cut up(chosen * tiles, (g.hidden + 63) / 64, g.sms, g.parts_up);
-    uint32_t hi[4], lo[4];
+    uint2 hi, lo;
     gated_values<T>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(lo_ai * tiles + k / 64),
                     static_cast<int64_t>(g.slots) * 2 * g.inner, hi, lo);
-    *reinterpret_cast<uint4 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint2 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = hi;
+    *reinterpret_cast<uint2 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = lo;
 }
 
-// One warp per 128 columns of one token, four per lane: the weighted parts, in ascending order within a choice, choices in
-// descending order of their logits. The warp first lists where they are, so that eight loads are in flight at a time.
 template <typename T>
 __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ MoeArgs g) {
     __shared__ int2 entry[4][B200_MOE_MAX_TOP_K * kMaxParts];
     const int t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tile = blockIdx.x * 4 + warp, n = tile * 128 + lane * 4;
-    const int tiles = (g.hidden + 127) / 128;
+    const int tile = blockIdx.x * 4 + warp, tiles = (g.hidden + 127) / 128;
     griddep_wait();
     griddep_launch_dependents();
     int slot = -1, parts = 0;
@@ -550,38 +739,12 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant_
         w = __ldcg(g.list.weight + at);
         if (slot >= 0 && tile < tiles) parts = cut.num_parts(__ldcg(g.list.active + at) * tiles + tile);
     }
-    int before = parts;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, before, 31);
-    for (int p = 0; p < parts; ++p) entry[warp][before - parts + p] = make_int2(p * g.slots + slot, __float_as_int(w));
-    __syncwarp();
-    if (n >= g.hidden) return;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i0 = 0; i0 < total; i0 += 8) {
-        float4 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i0 + i < total) v[i] = __ldcg(reinterpret_cast<const float4 *>(g.o + static_cast<int64_t>(entry[warp][i0 + i].x) * g.hidden + n));
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i0 + i < total) {
-                const float f = __int_as_float(entry[warp][i0 + i].y);
-                y.x = fmaf(f, v[i].x, y.x), y.y = fmaf(f, v[i].y, y.y), y.z = fmaf(f, v[i].z, y.z), y.w = fmaf(f, v[i].w, y.w);
-            }
-    }
-    uint2 out;
-    out.x = T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16;
-    out.y = T::round(y.z) | static_cast<uint32_t>(T::round(y.w)) << 16;
-    *reinterpret_cast<uint2 *>(g.Y + static_cast<int64_t>(t) * g.hidden + n) = out;
+    combine<T>(g, entry[warp], t, tile * 128 + lane * 4, lane, slot, parts, w);
 }
 
 int check_moe(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
     if (tokens <= 0 || tokens > B200_MOE_MAX_TOKENS || hidden <= 0 || inner <= 0 || hidden % 8 || inner % 8) return B200_INVALID_SHAPE;
-    if (hidden > 65536 || inner > 65536 || experts <= 0 || experts > B200_MOE_MAX_EXPERTS) return B200_INVALID_SHAPE;
+    if (hidden > kMaxHidden || inner > kMaxHidden || experts <= 0 || experts > B200_MOE_MAX_EXPERTS) return B200_INVALID_SHAPE;
     if (top_k < 1 || top_k > B200_MOE_MAX_TOP_K || top_k > experts) return B200_INVALID_CONFIG;
     return B200_OK;
 }
@@ -598,8 +761,8 @@ int most_parts(int64_t units, int64_t kblocks) {
 
 struct MoeLayout {
     int parts_up, parts_down;
-    bool gate_kernel;
-    int64_t off_list, off_z, off_o, off_h, bytes;
+    bool few;
+    int64_t off_list, off_z, off_o, off_h, bytes;   // few: the list is the counters of the tiles
 };
 
 MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
@@ -608,58 +771,57 @@ MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t expe
     l.parts_up = most_parts(top_k * up_tiles, (hidden + 63) / 64);
     l.parts_down = most_parts(top_k * ((hidden + 127) / 128), up_tiles);
     l.off_list = 0;
-    l.off_z = up256((2 + 3 * experts + 4 * slots) * 4);
+    l.few = slots <= kFewSlots && tokens <= kFewTokens;
+    l.off_z = l.few ? up256((hidden + 127) / 128 * 4) : up256((2 + 3 * experts + 4 * slots) * 4);
     l.off_o = l.off_z + up256(l.parts_up * slots * 2 * inner * 4);
     l.off_h = l.off_o + up256(l.parts_down * slots * hidden * 4);
-    l.gate_kernel = tokens > kFewTokens;
-    l.bytes = l.off_h + (l.gate_kernel ? up256(2 * slots * inner * 2) : 0);
+    l.bytes = l.off_h + (l.few ? 0 : up256(2 * slots * inner * 2));
     return l;
 }
 
-template <typename T>
-cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, bool gate_kernel, int smem, cudaStream_t stream) {
+template <typename Kernel>
+cudaError_t launch(Kernel *kernel, const MoeArgs &g, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    cfg.gridDim = dim3((g.tokens + 31) / 32);
-    cfg.blockDim = dim3(1024);
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cfg.gridDim.x;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, moe_route_kernel, g);
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(g.sms);
-    cfg.blockDim = dim3(kMoeThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, g);
+}
+
+template <typename T>
+cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, bool few, int smem, cudaStream_t stream) {
     g.map = up;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_product_kernel<T, UP>, g);
-    if (gate_kernel) {
-        cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(g.slots) * (g.inner / 8) + 255) / 256));
-        cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = 0;
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_gate_kernel<T>, g);
+    if (few) {
+        const cudaError_t e = launch(moe_product_kernel<T, UP_FEW>, g, g.sms, kMoeThreads, smem, 0, stream);
+        if (e != cudaSuccess) return e;
+        g.map = down;
+        return launch(moe_product_kernel<T, DOWN_FEW>, g, g.sms, kMoeThreads, smem, 0, stream);
     }
-    cfg.gridDim = dim3(g.sms);
-    cfg.blockDim = dim3(kMoeThreads);
-    cfg.dynamicSmemBytes = smem;
+    const int blocks = (g.tokens + 31) / 32;
+    cudaError_t e = launch(moe_route_kernel, g, blocks, 1024, 0, blocks, stream);
+    if (e == cudaSuccess) e = launch(moe_product_kernel<T, UP>, g, g.sms, kMoeThreads, smem, 0, stream);
+    const int64_t chunks = static_cast<int64_t>(g.slots) * (g.inner / 4);
+    if (e == cudaSuccess) e = launch(moe_gate_kernel<T>, g, static_cast<unsigned>((chunks + 255) / 256), 256, 0, 0, stream);
     g.map = down;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, gate_kernel ? moe_product_kernel<T, DOWN> : moe_product_kernel<T, DOWN_INLINE>, g);
-    cfg.gridDim = dim3((g.hidden + 511) / 512, g.tokens);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 0;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, moe_combine_kernel<T>, g);
+    if (e == cudaSuccess) e = launch(moe_product_kernel<T, DOWN>, g, g.sms, kMoeThreads, smem, 0, stream);
+    if (e == cudaSuccess) e = launch(moe_combine_kernel<T>, g, dim3((g.hidden + 511) / 512, g.tokens), 128, 0, 0, stream);
     return e;
 }
 
 }  // namespace
 
 int prepare_moe_kernels() {
-    void (*const kernels[])(MoeArgs) = {moe_product_kernel<Bf16, UP>, moe_product_kernel<Bf16, DOWN_INLINE>, moe_product_kernel<Bf16, DOWN>,
-                                        moe_product_kernel<Fp16, UP>, moe_product_kernel<Fp16, DOWN_INLINE>, moe_product_kernel<Fp16, DOWN>};
+    void (*const kernels[])(MoeArgs) = {moe_product_kernel<Bf16, UP>, moe_product_kernel<Bf16, DOWN>, moe_product_kernel<Bf16, UP_FEW>, moe_product_kernel<Bf16, DOWN_FEW>,
+                                        moe_product_kernel<Fp16, UP>, moe_product_kernel<Fp16, DOWN>, moe_product_kernel<Fp16, UP_FEW>, moe_product_kernel<Fp16, DOWN_FEW>};
     for (const auto k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
@@ -706,9 +868,10 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     const int64_t slots = tokens * top_k;
     g.h = reinterpret_cast<uint16_t *>(ws + l.off_h);
-    if (st == B200_OK && l.gate_kernel) st = encode_operand_map(&g.map_h, dtype, g.h, inner, 2 * slots, 16);
+    if (st == B200_OK && !l.few) st = encode_operand_map(&g.map_h, dtype, g.h, inner, 2 * slots, 16);
     if (st != B200_OK) return st;
     int *const list = reinterpret_cast<int *>(ws + l.off_list);
+    g.arrived = list;
     g.list.header = list;
     g.list.expert = list + 2;
     g.list.count = g.list.expert + experts;
@@ -737,16 +900,17 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     // so that DOWN can start beside UP; more tokens need the larger ring (a K block of DOWN is up to 80 KB then).
     g.slot_cols = static_cast<int>((tokens + 15) / 16 * 16);
     g.tmem_cols = pow2_at_least(2 * g.slot_cols);
-    const int lists = static_cast<int>(up256(slots * 2) + up256(experts * 12));
-    const int smem = tokens <= kFewTokens ? 113 * 1024 : kSmemLimit;
-    g.ring_bytes = (smem - 1024 - lists - 512) / 1024 * 1024;
-    g.off_token = g.ring_bytes;
-    g.off_expert = g.off_token + static_cast<int>(up256(slots * 2));
-    g.off_bars = g.ring_bytes + lists;
+    const int slot_lists = static_cast<int>(up256(slots * (l.few ? 10 : 2)));
+    const int expert_lists = static_cast<int>(up256(experts * (12 + (l.few ? (tokens + 31) / 32 * 4 + 2 : 0))));
+    const int smem = l.few ? 113 * 1024 : kSmemLimit;   // two blocks of 114 KB each are an SM's 228
+    g.ring_bytes = (smem - 1024 - slot_lists - expert_lists - 512) / 1024 * 1024;
+    g.off_slots = g.ring_bytes;
+    g.off_experts = g.off_slots + slot_lists;
+    g.off_bars = g.off_experts + expert_lists;
     g.off_misc = g.off_bars + (2 * kMoeStages + 4) * 8;
     g.idesc = umma_idesc(128, 0, dtype == B200_BF16);
     g.budget = wait_budget_cycles();
-    const cudaError_t e = dtype == B200_BF16 ? launch_moe<Bf16>(g, up, down, l.gate_kernel, smem, static_cast<cudaStream_t>(stream))
-                                             : launch_moe<Fp16>(g, up, down, l.gate_kernel, smem, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = dtype == B200_BF16 ? launch_moe<Bf16>(g, up, down, l.few, smem, static_cast<cudaStream_t>(stream))
+                                             : launch_moe<Fp16>(g, up, down, l.few, smem, static_cast<cudaStream_t>(stream));
     return e != cudaSuccess ? record_cuda_error(e) : B200_OK;
 }

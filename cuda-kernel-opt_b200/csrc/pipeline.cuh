@@ -63,6 +63,10 @@ __device__ __forceinline__ void st_shared_v4(uint32_t dst, const uint4 &v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_v2(uint32_t dst, const uint2 &v) {
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(v.x), "r"(v.y) : "memory");
+}
+
 // Byte offset of 16-byte chunk `chunk` of row `row` in a K block of 128-byte rows as TMA writes it with the 128-byte
 // swizzle (the chunk index is exclusive-ored with the row's place in its group of eight).
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
