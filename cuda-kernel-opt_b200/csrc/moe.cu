@@ -80,17 +80,6 @@ struct alignas(64) MoeArgs {
     long long budget;
 };
 
-// How the K blocks of `units` tiles are dealt out: CTA c takes blocks [c * len, (c + 1) * len) of all of them in a row. len is
-// large enough for a tile to touch at most `parts` CTAs.
-struct Cut {
-    int kblocks, total, len;
-    __device__ __forceinline__ Cut(int units, int kblocks_, int sms, int parts) : kblocks(kblocks_), total(units * kblocks_) {
-        len = max(max((total + sms - 1) / sms, (kblocks - 1 + parts - 2) / (parts - 1)), 1);
-    }
-    __device__ __forceinline__ int first_cta(int unit) const { return unit * kblocks / len; }
-    __device__ __forceinline__ int num_parts(int unit) const { return ((unit + 1) * kblocks - 1) / len - first_cta(unit) + 1; }
-};
-
 // Order-preserving map of a logit to an unsigned key; 0 = never chosen (-infinity, NaN). Equal floats (+-0 among
 // them) get equal keys; +infinity counts as the largest finite value.
 __device__ __forceinline__ uint32_t logit_key(float v) {

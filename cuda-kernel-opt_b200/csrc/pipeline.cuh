@@ -53,6 +53,17 @@ __device__ __forceinline__ void red_or_cluster(uint32_t cluster_addr, uint32_t b
     asm volatile("red.shared::cluster.or.b32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
 }
 
+// Completes `bar` when the MMAs issued before have; for a pair (the two CTAs of a cluster) the barrier at this place in both.
+template <int CG>
+__device__ __forceinline__ void commit_cta(uint32_t bar) {
+    if constexpr (CG == 1)
+        umma_commit<1>(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"(static_cast<uint16_t>(3))
+                     : "memory");
+}
+
 // 16 bytes global -> shared without passing through registers (L2 only); complete after cp_async_wait_all.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -72,5 +83,17 @@ __device__ __forceinline__ void st_shared_v2(uint32_t dst, const uint2 &v) {
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
     return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
 }
+
+// How the K blocks of `units` tiles are dealt out: CTA c takes blocks
+// [c * len, (c + 1) * len) of all of them in a row, wherever tiles begin and end. len is
+// large enough for a tile to touch at most `parts` CTAs.
+struct Cut {
+    int kblocks, total, len;
+    __device__ __forceinline__ Cut(int units, int kblocks_, int sms, int parts) : kblocks(kblocks_), total(units * kblocks_) {
+        len = max(max((total + sms - 1) / sms, (kblocks - 1 + parts - 2) / (parts - 1)), 1);
+    }
+    __device__ __forceinline__ int first_cta(int unit) const { return unit * kblocks / len; }
+    __device__ __forceinline__ int num_parts(int unit) const { return ((unit + 1) * kblocks - 1) / len - first_cta(unit) + 1; }
+};
 
 }  // namespace b200
