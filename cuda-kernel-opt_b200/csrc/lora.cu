@@ -35,7 +35,7 @@ constexpr int kLoraStages = 12;
 constexpr int kDeltaWarps = 8;
 constexpr int kLoraThreads = (2 + 4 + kDeltaWarps) * 32;
 constexpr int kChunkRows = 8;                              // rows of D in a piece of the adapters' product
-constexpr int kChunks = 8;                                 // pieces in flight
+constexpr int kChunks = 4;                                 // pieces in flight
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
 constexpr int kFewRows = 256;                              // most rows of the one-CTA form
 constexpr int kDotRows = 128;                              // most rows of the dot-product form of the shrink kernel
@@ -57,7 +57,7 @@ struct alignas(64) LoraArgs {
     int num_adapters;
     int parts, sms;
     int rows;                      // of a tile: columns of an accumulator
-    int a_bytes, stages, off_delta, off_bars, off_misc;
+    int a_bytes, stages, off_delta, off_u, off_bars, off_misc;
     int tmem_cols;
     uint32_t idesc;
     int *status;
@@ -218,50 +218,36 @@ struct LoraWalker {
     }
 };
 
-// One column n of D, rows m .. m + 3: sum over the ranks of u[row][r] * lora_b[s][n][r], fp32. Rows with the same adapter as the row before
-// find its 64 ranks at hand as floats (`held`, `kept`: whose they are); the others are read in blocks of 16 ranks.
+// One column n of D, four rows: sum over the ranks of u[j][r] * lora_b[s[j]][n][r], fp32, two ranks at a time. u lies in shared memory.
+// Where the four rows have one adapter, its ranks are kept as floats from one call to the next (h.w, h.s: whose they
+// are; up to 64 of them): a prompt's rows cost 32 packed multiply-adds each. Else every row's are read, 32 ranks at a
+// time: 16 loads of 16 bytes in flight per lane, which is what reading each adapter once from memory takes.
 struct Held {
     float2 w[32];
     int s;
 };
 
 template <typename T>
-__device__ __forceinline__ void hold(const LoraArgs &g, Held &h, int s, int n) {
-    const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s) * g.N + n) * g.rank);
+__device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, const int (&s)[4], const float *u, int n, float (&d)[4]) {
+    const int rank = g.rank;
+    if (s[0] >= 0 && s[0] == s[1] && s[0] == s[2] && s[0] == s[3] && rank <= 64) {
+        if (h.s != s[0]) {
+            const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[0]) * g.N + n) * rank);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint4 v = i * 8 < g.rank ? __ldcg(b + i) : make_uint4(0, 0, 0, 0);
-        h.w[4 * i] = T::unpack(v.x), h.w[4 * i + 1] = T::unpack(v.y), h.w[4 * i + 2] = T::unpack(v.z), h.w[4 * i + 3] = T::unpack(v.w);
-    }
-    h.s = s;
-}
-
-template <typename T>
-__device__ __forceinline__ float fma16(const LoraArgs &g, const uint4 &b0, const uint4 &b1, const float *u, bool second, float acc) {
-    const uint32_t b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i == 2 && !second) break;
-        const float4 f = __ldca(reinterpret_cast<const float4 *>(u) + i);
-        const float2 p = T::unpack(b[2 * i]), q = T::unpack(b[2 * i + 1]);
-        acc = fmaf(f.x, p.x, fmaf(f.y, p.y, fmaf(f.z, q.x, fmaf(f.w, q.y, acc))));
-    }
-    return acc;
-}
-
-template <typename T>
-__device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, const int (&s)[4], int m, int n, float (&d)[4]) {
-    const bool same = s[0] >= 0 && s[0] == s[1] && s[0] == s[2] && s[0] == s[3];
-    if (same && g.rank <= 64) {
-        if (h.s != s[0]) hold<T>(g, h, s[0], n);
+            for (int i = 0; i < 8; ++i) {
+                const uint4 v = i * 8 < rank ? __ldcg(b + i) : make_uint4(0, 0, 0, 0);
+                h.w[4 * i] = T::unpack(v.x), h.w[4 * i + 1] = T::unpack(v.y), h.w[4 * i + 2] = T::unpack(v.z), h.w[4 * i + 3] = T::unpack(v.w);
+            }
+            h.s = s[0];
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float4 *const u = reinterpret_cast<const float4 *>(g.u + static_cast<int64_t>(m + j) * g.rank);
+            const float4 *const uj = reinterpret_cast<const float4 *>(u + j * rank);
             float2 a = make_float2(0.0f, 0.0f), b = a;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                if (i * 4 >= g.rank) break;
-                const float4 f = __ldca(u + i), e = __ldca(u + i + 1);
+                if (i * 4 >= rank) break;
+                const float4 f = uj[i], e = uj[i + 1];
                 a = fma2(make_float2(f.x, f.y), h.w[2 * i], a);
                 b = fma2(make_float2(f.z, f.w), h.w[2 * i + 1], b);
                 a = fma2(make_float2(e.x, e.y), h.w[2 * i + 2], a);
@@ -271,22 +257,60 @@ __device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, con
         }
         return;
     }
+    h.s = -1;                                              // its place takes the rows' elements as they were read
+    float2 sum[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = 0.0f;
-    for (int r = 0; r < g.rank; r += 16) {
-        const bool second = r + 8 < g.rank;
-        uint4 b[4][2];
+    for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    for (int r = 0; r < rank; r += 32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint4 *const p = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[j]) * g.N + n) * g.rank + r);
-            if (s[j] >= 0) b[j][0] = __ldcg(p);
-            if (s[j] >= 0 && second) b[j][1] = __ldcg(p + 1);
+            const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[j]) * g.N + n) * rank + r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 v = s[j] >= 0 && r + 8 * i < rank ? __ldcg(b + i) : make_uint4(0, 0, 0, 0);
+                h.w[8 * j + 2 * i] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+                h.w[8 * j + 2 * i + 1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (s[j] >= 0) d[j] = fma16<T>(g, b[j][0], b[j][1], g.u + static_cast<int64_t>(m + j) * g.rank + r, second, d[j]);
+        for (int j = 0; j < 4; ++j) {
+            if (s[j] < 0) continue;
+            const float4 *const uj = reinterpret_cast<const float4 *>(u + j * rank + r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (r + 8 * i >= rank) break;
+                const float4 f = uj[2 * i], e = uj[2 * i + 1];
+                sum[j] = fma2(make_float2(f.x, f.y), T::unpack(__float_as_uint(h.w[8 * j + 2 * i].x)), sum[j]);
+                sum[j] = fma2(make_float2(f.z, f.w), T::unpack(__float_as_uint(h.w[8 * j + 2 * i].y)), sum[j]);
+                sum[j] = fma2(make_float2(e.x, e.y), T::unpack(__float_as_uint(h.w[8 * j + 2 * i + 1].x)), sum[j]);
+                sum[j] = fma2(make_float2(e.z, e.w), T::unpack(__float_as_uint(h.w[8 * j + 2 * i + 1].y)), sum[j]);
+            }
+        }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = sum[j].x + sum[j].y;
 }
+
+// The pieces of one CTA's adapters' product in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
+template <int CG>
+struct PieceWalker {
+    LoraWalker<CG> walk;
+    LoraSegment s;
+    int c, rows;
+    __device__ __forceinline__ PieceWalker(const LoraWalker<CG> &w) : walk(w) {
+        c = rows = 0;
+        s.parts = 0;
+    }
+    __device__ __forceinline__ bool next(const LoraArgs &g) {
+        c += s.parts;
+        while (c * kChunkRows >= rows) {
+            if (!walk.next(s)) return false;
+            rows = min(g.rows, g.M - s.m0);
+            c = s.part;
+        }
+        return true;
+    }
+};
 
 template <typename T, int CG>
 __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __grid_constant__ LoraArgs g) {
@@ -454,32 +478,48 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     } else {
         // -------------------------------------------------------------- the adapters' product
         const int t = tid - 6 * 32, n = t & 127, half = (t >> 7) * 4;
+        float *const u_s = reinterpret_cast<float *>(sm + g.off_u) + (warp - 6) * 4 * g.rank;   // this warp's four rows
         Held held;
         held.s = -1;
-        int piece = 0, held_col = -1;
-        griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
-        while (ok && walk.next(s)) {
-            const int rows = min(g.rows, g.M - s.m0);
-            const int col = (s.tile * CG + static_cast<int>(rank)) * 128 + n;
-            if (col != held_col) held.s = -1, held_col = col;
-            for (int c = s.part; c * kChunkRows < rows; c += s.parts, ++piece) {
-                const int slot = piece % kChunks, m = s.m0 + c * kChunkRows + half;
-                int id[4];
+        int held_col = -1, id[4];
+        float4 u[4];
+        PieceWalker<CG> at(walk);
+        // Adapters and u of a piece are read while the piece before it is computed.
+        auto fetch = [&] {
+            const int m = at.s.m0 + at.c * kChunkRows + half;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int v = m + j < g.M ? __ldca(g.row_adapter + m + j) : -1;
-                    id[j] = static_cast<unsigned>(v) < static_cast<unsigned>(g.num_adapters) ? v : -1;
-                }
-                float d[4] = {};
-                if (col < g.N) adapters_product<T>(g, held, id, m, col, d);
-                __syncwarp();
-                ok = wait_warp(delta_empty0 + 8 * slot, ((piece / kChunks) & 1) ^ 1u, wait, 2500 + slot);
-                if (!ok) break;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) delta[(slot * kChunkRows + half + j) * 128 + n] = d[j];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(delta_full0 + 8 * slot);
+            for (int j = 0; j < 4; ++j) {
+                const int v = m + j < g.M ? __ldca(g.row_adapter + m + j) : -1;
+                id[j] = static_cast<unsigned>(v) < static_cast<unsigned>(g.num_adapters) ? v : -1;
             }
+            const int count = min(4, g.M - m) * (g.rank / 4);   // the four rows lie behind one another
+            const float4 *const src = reinterpret_cast<const float4 *>(g.u + static_cast<int64_t>(m) * g.rank);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (lane + 32 * i < count) u[i] = __ldcg(src + lane + 32 * i);
+        };
+        griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
+        bool more = at.next(g);
+        if (more) fetch();
+        for (int piece = 0; ok && more; ++piece) {
+            const int slot = piece % kChunks, col = (at.s.tile * CG + static_cast<int>(rank)) * 128 + n;
+            if (col != held_col) held.s = -1, held_col = col;
+            const int now[4] = {id[0], id[1], id[2], id[3]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (lane + 32 * i < g.rank) reinterpret_cast<float4 *>(u_s)[lane + 32 * i] = u[i];
+            __syncwarp();
+            more = at.next(g);
+            if (more) fetch();
+            float d[4] = {};
+            if (col < g.N) adapters_product<T>(g, held, now, u_s, col, d);
+            __syncwarp();
+            ok = wait_warp(delta_empty0 + 8 * slot, ((piece / kChunks) & 1) ^ 1u, wait, 2500 + slot);
+            if (!ok) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) delta[(slot * kChunkRows + half + j) * 128 + n] = d[j];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(delta_full0 + 8 * slot);
         }
     }
 
@@ -655,12 +695,13 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     if (st == B200_OK) st = encode_operand_map(&g.map_a, dtype, A, K, M, box_a);
     if (st != B200_OK) return st;
     g.a_bytes = box_a * 128;
-    const int rest = kChunks * kChunkBytes + (2 * kLoraStages + 4 + 2 * kChunks) * 8 + 16;
+    const int rest = kChunks * kChunkBytes + kDeltaWarps * 4 * rank * 4 + (2 * kLoraStages + 4 + 2 * kChunks) * 8 + 16;
     // one CTA: 32 KB of the SM stay free for blocks of the shrink kernel
     g.stages = ((pair ? kSmemLimit : 196 * 1024) - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
-    g.off_bars = g.off_delta + kChunks * kChunkBytes;
+    g.off_u = g.off_delta + kChunks * kChunkBytes;
+    g.off_bars = g.off_u + kDeltaWarps * 4 * rank * 4;
     g.off_misc = g.off_bars + (2 * kLoraStages + 4 + 2 * kChunks) * 8;
     const int smem = 1024 + g.off_delta + rest;
     g.tmem_cols = pow2_at_least(2 * g.rows);
