@@ -33,12 +33,15 @@ namespace {
 
 constexpr int kLoraStages = 12;
 constexpr int kDeltaWarps = 8;
-constexpr int kLoraThreads = (2 + 4 + kDeltaWarps) * 32;
+constexpr int kLoraThreads = (2 + 4 + kDeltaWarps + 1) * 32;
 constexpr int kChunkRows = 8;                              // rows of D in a piece of the adapters' product
-constexpr int kChunks = 4;                                 // pieces in flight
+constexpr int kChunks = 4;                                 // pieces on their way to the draining warps
+constexpr int kAhead = 8;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
-constexpr int kFewRows = 256;                              // most rows of the one-CTA form
+constexpr int kOneCtaRows = 64;                            // most rows of the one-CTA form
+constexpr int kFewRows = 256;                              // most rows that one tile takes
 constexpr int kDotRows = 128;                              // most rows of the dot-product form of the shrink kernel
+constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kChunks + 2 * kAhead;
 constexpr int kMaxLoraParts = 16;
 constexpr int kMaxCtas = 256;
 constexpr int kLoraGridSms = 148;                          // what the workspace is sized for
@@ -55,9 +58,10 @@ struct alignas(64) LoraArgs {
     int *arrived;                  // per CTA: the warps that are done with the tile it began last
     int M, N, K, rank;
     int num_adapters;
+    int wide_b;                    // rows of lora_b are whole 32-byte sectors
     int parts, sms;
     int rows;                      // of a tile: columns of an accumulator
-    int a_bytes, stages, off_delta, off_u, off_bars, off_misc;
+    int a_bytes, stages, off_delta, off_u, off_ids, off_bars, off_misc;
     int tmem_cols;
     uint32_t idesc;
     int *status;
@@ -177,30 +181,30 @@ struct LoraSegment {
     int tile, m0, kb0, kb1, part, parts;
 };
 
-template <int CG>
+template <int CG, bool WAVES>
 struct LoraWalker {
-    int q, end, step, tiles_n, row_blocks, kblocks, rows, cta;
+    int q, end, step, tiles_n, row_blocks, kblocks, rows, group;   // group: a CTA or a pair
     Cut cut;
     __device__ __forceinline__ LoraWalker(const LoraArgs &g)
         : tiles_n((g.N + 128 * CG - 1) / (128 * CG)), row_blocks((g.M + g.rows - 1) / g.rows), kblocks((g.K + 63) / 64), rows(g.rows),
-          cta(blockIdx.x), cut(CG == 1 ? tiles_n : 0, kblocks, g.sms, g.parts) {
-        if (CG == 1) {
-            q = static_cast<int>(min(static_cast<long long>(cta) * cut.len, static_cast<long long>(cut.total)));
-            end = min(q + cut.len, cut.total);
-        } else {
-            q = blockIdx.x / 2;
-            step = gridDim.x / 2;
+          group(blockIdx.x / CG), cut(WAVES ? 0 : tiles_n, kblocks, gridDim.x / CG, g.parts) {
+        if (WAVES) {
+            q = group;
+            step = gridDim.x / CG;
             end = tiles_n * row_blocks;
+        } else {
+            q = static_cast<int>(min(static_cast<long long>(group) * cut.len, static_cast<long long>(cut.total)));
+            end = min(q + cut.len, cut.total);
         }
     }
     __device__ __forceinline__ bool next(LoraSegment &s) {
         if (q >= end) return false;
-        if (CG == 1) {
+        if (!WAVES) {
             s.tile = q / kblocks;
             s.m0 = 0;
             s.kb0 = q - s.tile * kblocks;
             s.kb1 = min(kblocks, s.kb0 + end - q);
-            s.part = cta - cut.first_cta(s.tile);
+            s.part = group - cut.first_cta(s.tile);
             s.parts = cut.num_parts(s.tile);
             q += s.kb1 - s.kb0;
         } else {
@@ -257,6 +261,7 @@ __device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, con
         }
         return;
     }
+    const bool wide = g.wide_b != 0;
     h.s = -1;                                              // its place takes the rows' elements as they were read
     float2 sum[4];
 #pragma unroll
@@ -266,10 +271,19 @@ __device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, con
         for (int j = 0; j < 4; ++j) {
             const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[j]) * g.N + n) * rank + r);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 v = s[j] >= 0 && r + 8 * i < rank ? __ldcg(b + i) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 4; i += 2) {
+                uint4 v = make_uint4(0, 0, 0, 0), w = v;
+                if (s[j] >= 0 && r + 8 * i < rank) {
+                    if (wide) ld_32(b + i, v, w);          // a whole sector per lane
+                    else {
+                        v = __ldcg(b + i);
+                        if (r + 8 * i + 8 < rank) w = __ldcg(b + i + 1);
+                    }
+                }
                 h.w[8 * j + 2 * i] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
                 h.w[8 * j + 2 * i + 1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+                h.w[8 * j + 2 * i + 2] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+                h.w[8 * j + 2 * i + 3] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
             }
         }
 #pragma unroll
@@ -292,12 +306,12 @@ __device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, con
 }
 
 // The pieces of one CTA's adapters' product in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
-template <int CG>
+template <int CG, bool WAVES>
 struct PieceWalker {
-    LoraWalker<CG> walk;
+    LoraWalker<CG, WAVES> walk;
     LoraSegment s;
     int c, rows;
-    __device__ __forceinline__ PieceWalker(const LoraWalker<CG> &w) : walk(w) {
+    __device__ __forceinline__ PieceWalker(const LoraWalker<CG, WAVES> &w) : walk(w) {
         c = rows = 0;
         s.parts = 0;
     }
@@ -312,24 +326,28 @@ struct PieceWalker {
     }
 };
 
-template <typename T, int CG>
+template <typename T, int CG, bool WAVES>
 __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __grid_constant__ LoraArgs g) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t *const sm = smem_raw + (ring - raw);
     float *const delta = reinterpret_cast<float *>(sm + g.off_delta);
+    float *const u_s = reinterpret_cast<float *>(sm + g.off_u);
+    int *const id_s = reinterpret_cast<int *>(sm + g.off_ids);
     const uint32_t full0 = ring + g.off_bars, empty0 = full0 + 8 * kLoraStages, acc_full0 = empty0 + 8 * kLoraStages, acc_empty0 = acc_full0 + 16,
-                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kChunks;
+                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kChunks,
+                   u_full0 = delta_empty0 + 8 * kChunks, u_empty0 = u_full0 + 8 * kAhead;
     volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // abort flag, tensor-memory base, two tiles whose parts this CTA adds
     const WaitCtx wait = {g.status, misc, g.budget};
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t rank = CG == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
 
-    if (tid < 2 * kLoraStages + 4 + 2 * kChunks) {
-        const int j = tid - 2 * kLoraStages;
-        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kChunks ? kDeltaWarps : 4);
+    if (tid < kLoraBars) {
+        // accumulators: full, empty (the draining warps of the pair); pieces: full (the delta warps), empty (the draining warps); u: full, empty
+        const int j = tid - 2 * kLoraStages, i = j - 4 - 2 * kChunks;
+        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kChunks ? kDeltaWarps : i < 0 ? 4 : i < kAhead ? 1 : kDeltaWarps);
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0, misc[2] = misc[3] = -1;
@@ -354,7 +372,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     constexpr int kBBytes = 128 * 128;                     // 128 rows of B, 64 elements of K
     const uint32_t stage_bytes = kBBytes + g.a_bytes;
     const int stages = g.stages;
-    LoraWalker<CG> walk(g);
+    LoraWalker<CG, WAVES> walk(g);
     LoraSegment s;
     int st = 0;
     uint32_t ph = 0;
@@ -364,10 +382,10 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         // -------------------------------------------------------------- operands: TMA
         const bool issuer = elect_one();
         const uint32_t full_leader = CG == 2 ? __shfl_sync(0xffffffffu, mapa_shared(full0, 0), 0) : full0;
-        const uint64_t pol_b = l2_policy(CG == 1 ? 1 : 2), pol_a = l2_policy(2);
+        const uint64_t pol_b = l2_policy(WAVES ? 2 : 1), pol_a = l2_policy(2);
         for (int n = 0; ok && walk.next(s); ++n) {
-            const int row_b = (s.tile * CG + static_cast<int>(rank)) * 128, row_a = s.m0 + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
-            const bool down = CG == 2 && (n & 1);          // to and fro: the panel ends touched last are still in L2
+            const int row_b = (s.tile * CG + static_cast<int>(rank)) * 128, row_a = s.m0 + static_cast<int>(rank) * (g.rows / CG);
+            const bool down = WAVES && (n & 1);          // to and fro: the panel ends touched last are still in L2
             for (int i = s.kb0; i < s.kb1; ++i) {
                 ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 2000 + st);
                 if (!ok) break;
@@ -464,62 +482,60 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 if constexpr (CG == 2) mbar_arrive_cluster(acc_empty_leader + 8 * acc);
                 else mbar_arrive(acc_empty0 + 8 * acc);
             }
-            if (CG == 1 && s.parts > 1) {
-                // Four warps of each CTA of the tile count, under the number of the CTA that began the tile (no CTA begins two
-                // that it does not finish); the CTA whose warp is the last one adds the parts in the end.
+            if (!WAVES && s.parts > 1) {
+                // Four warps of each CTA of the tile's columns count, under the number of the CTA that began them (no CTA begins
+                // two tiles that it does not finish); the CTA whose warp is the last one adds the parts in the end.
                 __threadfence();
                 __syncwarp();
-                if (lane == 0 && atomicAdd(g.arrived + walk.cta - s.part, 1) == 4 * s.parts - 1) {
+                if (lane == 0 && atomicAdd(g.arrived + blockIdx.x - CG * s.part, 1) == 4 * s.parts - 1) {
                     __threadfence();
                     misc[s.kb0 > 0 ? 2 : 3] = s.tile;
                 }
             }
         }
-    } else {
+    } else if (warp < 6 + kDeltaWarps) {
         // -------------------------------------------------------------- the adapters' product
         const int t = tid - 6 * 32, n = t & 127, half = (t >> 7) * 4;
-        float *const u_s = reinterpret_cast<float *>(sm + g.off_u) + (warp - 6) * 4 * g.rank;   // this warp's four rows
         Held held;
         held.s = -1;
-        int held_col = -1, id[4];
-        float4 u[4];
-        PieceWalker<CG> at(walk);
-        // Adapters and u of a piece are read while the piece before it is computed.
-        auto fetch = [&] {
-            const int m = at.s.m0 + at.c * kChunkRows + half;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = m + j < g.M ? __ldca(g.row_adapter + m + j) : -1;
-                id[j] = static_cast<unsigned>(v) < static_cast<unsigned>(g.num_adapters) ? v : -1;
-            }
-            const int count = min(4, g.M - m) * (g.rank / 4);   // the four rows lie behind one another
-            const float4 *const src = reinterpret_cast<const float4 *>(g.u + static_cast<int64_t>(m) * g.rank);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < count) u[i] = __ldcg(src + lane + 32 * i);
-        };
-        griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
-        bool more = at.next(g);
-        if (more) fetch();
-        for (int piece = 0; ok && more; ++piece) {
-            const int slot = piece % kChunks, col = (at.s.tile * CG + static_cast<int>(rank)) * 128 + n;
+        int held_col = -1;
+        PieceWalker<CG, WAVES> at(walk);
+        griddep_wait();                                    // nothing that this SM's first-level cache may hold is older than the operands
+        for (int piece = 0; ok && at.next(g); ++piece) {
+            const int slot = piece % kChunks, from = piece % kAhead, col = (at.s.tile * CG + static_cast<int>(rank)) * 128 + n;
             if (col != held_col) held.s = -1, held_col = col;
-            const int now[4] = {id[0], id[1], id[2], id[3]};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < g.rank) reinterpret_cast<float4 *>(u_s)[lane + 32 * i] = u[i];
-            __syncwarp();
-            more = at.next(g);
-            if (more) fetch();
+            ok = wait_warp(u_full0 + 8 * from, (piece / kAhead) & 1, wait, 2600 + from);
+            if (!ok) break;
+            const int4 q = *reinterpret_cast<const int4 *>(id_s + from * kChunkRows + half);
+            const int id[4] = {q.x, q.y, q.z, q.w};
             float d[4] = {};
-            if (col < g.N) adapters_product<T>(g, held, now, u_s, col, d);
+            if (col < g.N) adapters_product<T>(g, held, id, u_s + (from * kChunkRows + half) * g.rank, col, d);
             __syncwarp();
+            if (lane == 0) mbar_arrive(u_empty0 + 8 * from);
             ok = wait_warp(delta_empty0 + 8 * slot, ((piece / kChunks) & 1) ^ 1u, wait, 2500 + slot);
             if (!ok) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) delta[(slot * kChunkRows + half + j) * 128 + n] = d[j];
             __syncwarp();
             if (lane == 0) mbar_arrive(delta_full0 + 8 * slot);
+        }
+    } else {
+        // -------------------------------------------------------------- u and the rows' adapters for the warps above
+        PieceWalker<CG, WAVES> at(walk);
+        griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
+        for (int piece = 0; ok && at.next(g); ++piece) {
+            const int from = piece % kAhead, m = at.s.m0 + at.c * kChunkRows;
+            int id = -1;
+            if (lane < kChunkRows && m + lane < g.M) id = __ldca(g.row_adapter + m + lane);
+            ok = wait_warp(u_empty0 + 8 * from, ((piece / kAhead) & 1) ^ 1u, wait, 2700 + from);
+            if (!ok) break;
+            if (lane < kChunkRows) id_s[from * kChunkRows + lane] = static_cast<unsigned>(id) < static_cast<unsigned>(g.num_adapters) ? id : -1;
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t bytes = static_cast<uint32_t>(min(kChunkRows, g.M - m) * g.rank * 4);
+                mbar_arrive_expect_tx(u_full0 + 8 * from, bytes);
+                bulk_load(smem_u32(u_s + from * kChunkRows * g.rank), g.u + static_cast<int64_t>(m) * g.rank, bytes, u_full0 + 8 * from);
+            }
         }
     }
 
@@ -529,11 +545,11 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         cluster_arrive();
         cluster_wait();
     }
-    if (CG == 1 && !misc[0]) {
+    if (!WAVES && !misc[0]) {
         for (int i = 2; i < 4; ++i) {
             const int tile = misc[i];
             if (tile < 0) continue;
-            const int parts = walk.cut.num_parts(tile), col = tile * 128 + lane * 4;
+            const int parts = walk.cut.num_parts(tile), col = (tile * CG + static_cast<int>(rank)) * 128 + lane * 4;
             if (col >= g.N) continue;
             const int64_t pitch = static_cast<int64_t>(g.M) * g.N;
             for (int m = warp; m < g.M; m += kLoraThreads / 32) {
@@ -590,13 +606,14 @@ cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
         else e = launch(lora_shrink_mma_kernel<T, 1>, g, dim3(row_blocks, g.rank / 8), 256, 0, 1, stream);
     }
     if (e != cudaSuccess) return e;
-    if (g.M <= kFewRows) return launch(lora_product_kernel<T, 1>, g, g.sms, kLoraThreads, smem, 1, stream);
-    return launch(lora_product_kernel<T, 2>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
+    if (g.M <= kOneCtaRows) return launch(lora_product_kernel<T, 1, false>, g, g.sms, kLoraThreads, smem, 1, stream);
+    if (g.M <= kFewRows) return launch(lora_product_kernel<T, 2, false>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
+    return launch(lora_product_kernel<T, 2, true>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
 }
 
 // CTAs that may share a tile, one more for stretches that do not start at a tile.
-int most_parts(int64_t units, int64_t kblocks) {
-    const int64_t len = (units * kblocks + kLoraGridSms - 1) / kLoraGridSms;
+int most_parts(int64_t units, int64_t kblocks, int64_t groups) {
+    const int64_t len = (units * kblocks + groups - 1) / groups;
     const int64_t parts = (kblocks - 1 + len - 1) / len + 1;
     return static_cast<int>(parts < 2 ? 2 : parts > kMaxLoraParts ? kMaxLoraParts : parts);
 }
@@ -608,7 +625,7 @@ struct LoraLayout {
 
 LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int rank) {
     LoraLayout l;
-    l.parts = M <= kFewRows ? most_parts((N + 127) / 128, (K + 63) / 64) : 2;
+    l.parts = M > kFewRows ? 2 : M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
     l.off_u = kMaxCtas * 4;
     l.off_o = l.off_u + (M * rank * 4 + 255) / 256 * 256;
     l.bytes = l.off_o + (M <= kFewRows ? l.parts * M * N * 4 : 0);
@@ -627,7 +644,8 @@ int check_lora(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) 
 
 int prepare_moe_kernels();
 int prepare_routed_kernels() {
-    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, 1>, lora_product_kernel<Bf16, 2>, lora_product_kernel<Fp16, 1>, lora_product_kernel<Fp16, 2>};
+    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, 1, false>, lora_product_kernel<Bf16, 2, false>, lora_product_kernel<Bf16, 2, true>,
+                                         lora_product_kernel<Fp16, 1, false>, lora_product_kernel<Fp16, 2, false>, lora_product_kernel<Fp16, 2, true>};
     for (const auto k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
@@ -688,24 +706,26 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.rank = rank;
     g.num_adapters = static_cast<int>(num_adapters);
     g.parts = l.parts;
-    const bool pair = M > kFewRows;
-    g.rows = pair ? 256 : static_cast<int>((M + 15) / 16 * 16);
-    const int box_a = pair ? 128 : g.rows;
+    const int cg = M > kOneCtaRows ? 2 : 1;
+    g.rows = M > kFewRows ? 256 : static_cast<int>((M + 16 * cg - 1) / (16 * cg) * (16 * cg));
+    const int box_a = g.rows / cg;
+    g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
     st = encode_operand_map(&g.map_b, dtype, Bt, K, N, 128);
     if (st == B200_OK) st = encode_operand_map(&g.map_a, dtype, A, K, M, box_a);
     if (st != B200_OK) return st;
     g.a_bytes = box_a * 128;
-    const int rest = kChunks * kChunkBytes + kDeltaWarps * 4 * rank * 4 + (2 * kLoraStages + 4 + 2 * kChunks) * 8 + 16;
-    // one CTA: 32 KB of the SM stay free for blocks of the shrink kernel
-    g.stages = ((pair ? kSmemLimit : 196 * 1024) - 1024 - rest) / (128 * 128 + g.a_bytes);
+    const int u_bytes = kAhead * kChunkRows * rank * 4, rest = kChunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
+    // up to 256 rows 32 KB of the SM stay free for blocks of the shrink kernel
+    g.stages = ((M > kFewRows ? kSmemLimit : 196 * 1024) - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
     g.off_u = g.off_delta + kChunks * kChunkBytes;
-    g.off_bars = g.off_u + kDeltaWarps * 4 * rank * 4;
-    g.off_misc = g.off_bars + (2 * kLoraStages + 4 + 2 * kChunks) * 8;
+    g.off_ids = g.off_u + u_bytes;
+    g.off_bars = g.off_ids + kAhead * kChunkRows * 4;
+    g.off_misc = g.off_bars + kLoraBars * 8;
     const int smem = 1024 + g.off_delta + rest;
     g.tmem_cols = pow2_at_least(2 * g.rows);
-    g.idesc = umma_idesc(pair ? 256 : 128, g.rows, dtype == B200_BF16);
+    g.idesc = umma_idesc(128 * cg, g.rows, dtype == B200_BF16);
     g.budget = wait_budget_cycles();
     const cudaError_t e = dtype == B200_BF16 ? launch_lora<Bf16>(g, smem < kMinSmemRequest ? kMinSmemRequest : smem, static_cast<cudaStream_t>(stream))
                                              : launch_lora<Fp16>(g, smem < kMinSmemRequest ? kMinSmemRequest : smem, static_cast<cudaStream_t>(stream));

@@ -64,6 +64,12 @@ __device__ __forceinline__ void commit_cta(uint32_t bar) {
                      : "memory");
 }
 
+// Contiguous bytes global -> shared (both 16-byte aligned, a multiple of 16), counted by `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // 16 bytes global -> shared without passing through registers (L2 only); complete after cp_async_wait_all.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
