@@ -34,26 +34,37 @@ namespace {
 constexpr int kLoraStages = 12;
 constexpr int kDeltaWarps = 8;
 constexpr int kLoraThreads = (2 + 4 + kDeltaWarps + 1) * 32;
-constexpr int kChunkRows = 8;                              // rows of D in a piece of the adapters' product
-constexpr int kChunks = 4;                                 // pieces on their way to the draining warps
-constexpr int kAhead = 8;                                  // pieces whose adapters and u are on their way to the delta warps
+constexpr int kChunkRows = 16;                             // rows of D in a piece of the adapters' product
+constexpr int kMaxChunks = 8;                              // most pieces on their way to the draining warps
+constexpr int kAhead = 4;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
 constexpr int kOneCtaRows = 64;                            // most rows of the one-CTA form
 constexpr int kFewRows = 256;                              // most rows that one tile takes
-constexpr int kDotRows = 128;                              // most rows of the dot-product form of the shrink kernel
-constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kChunks + 2 * kAhead;
+constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kMaxChunks + 2 * kAhead;
+constexpr int kNoRow = -2;                                 // in the place of an adapter: behind the last row
 constexpr int kMaxLoraParts = 16;
 constexpr int kMaxCtas = 256;
+constexpr int kMaxBlocks = 256;                            // blocks of 256 rows of one pass; more rows are several passes
+constexpr int kGroup = 32;                                 // rows that share a way of adding their adapters
 constexpr int kLoraGridSms = 148;                          // what the workspace is sized for
 constexpr int kGroupRows = 16;                             // pair: row blocks that a wave walks together
 
 struct alignas(64) LoraArgs {
     CUtensorMap map_b, map_a;      // B as {K, N}, A as {K, M}
+    CUtensorMap map_la, map_lb, map_u;   // many rows: lora_a as {K, adapters * rank}, lora_b as {rank, adapters * N}, u16 as {rank, 2 * M}
     const uint16_t *A, *lora_a, *lora_b;
     uint16_t *D;
     const float *scale;
     const int *row_adapter;
     float *u;                      // [M][rank]
+    float *u_parts;                // [part][M][rank]
+    uint16_t *u16;                 // [value, remainder][M][rank]
+    struct {
+        int *count, *adapter, *entry;   // per block of 256 rows: adapters that occur, and which; per row: which of them it has
+        int *wide;                 // per 32 rows: some u does not fit a pair of 16-bit numbers
+    } list;
+    int parts_u, on_tensor;        // parts of u; whether the adapters' second product may use the tensor core
+    uint32_t idesc_u, idesc_run;   // run: with N = 0
     float *o;                      // [part][M][N]: sums of tiles that span CTAs
     int *arrived;                  // per CTA: the warps that are done with the tile it began last
     int M, N, K, rank;
@@ -61,12 +72,19 @@ struct alignas(64) LoraArgs {
     int wide_b;                    // rows of lora_b are whole 32-byte sectors
     int parts, sms;
     int rows;                      // of a tile: columns of an accumulator
+    int u_pitch, chunks;           // floats from row to row of u in shared memory; pieces in flight
     int a_bytes, stages, off_delta, off_u, off_ids, off_bars, off_misc;
     int tmem_cols;
     uint32_t idesc;
     int *status;
     long long budget;
 };
+
+__device__ __forceinline__ int row_adapter(const LoraArgs &g, int m) {   // -1: none, kNoRow: no such row
+    if (m >= g.M) return kNoRow;
+    const int s = __ldca(g.row_adapter + m);
+    return static_cast<unsigned>(s) < static_cast<unsigned>(g.num_adapters) ? s : -1;
+}
 
 // ---------------------------------------------------------------------------------------------- first product
 
@@ -82,8 +100,8 @@ __global__ void __launch_bounds__(256) lora_shrink_dot_kernel(const __grid_const
     const int quads = g.rank / 4;
     for (int64_t at = blockIdx.x; at < static_cast<int64_t>(g.M) * quads; at += gridDim.x) {
         const int m = static_cast<int>(at / quads), r0 = static_cast<int>(at - static_cast<int64_t>(m) * quads) * 4;
-        const int s = __ldca(g.row_adapter + m);
-        if (static_cast<unsigned>(s) >= static_cast<unsigned>(g.num_adapters)) continue;
+        const int s = row_adapter(g, m);
+        if (s < 0) continue;
         const uint16_t *const x = g.A + static_cast<int64_t>(m) * g.K;
         const uint16_t *const a = g.lora_a + (static_cast<int64_t>(s) * g.rank + r0) * g.K;
         float acc[4] = {};
@@ -112,66 +130,240 @@ __global__ void __launch_bounds__(256) lora_shrink_dot_kernel(const __grid_const
     }
 }
 
-// Many rows: a block takes 16 rows and 8 * NT ranks, its warps an eighth of the K steps of 32 each, on mma.sync (the rows of an
-// adapter are few and any; a 128-row tile of tcgen05 would be mostly other adapters' rows). One pass over K per adapter among
-// the 16 rows; only its own rows keep the result. Within a step the four lanes of a quad hold 8 neighbouring elements each, of both
-// operands alike: the order of K within a step is free.
-template <typename T, int NT>
-__global__ void __launch_bounds__(256) lora_shrink_mma_kernel(const __grid_constant__ LoraArgs g) {
-    __shared__ float sums[8][16][8 * NT];
-    __shared__ int ids[16];
+// More rows: lora_a's ranks on the 128-row side of tcgen05.mma, 256 rows of A as its columns, one product per block of rows and adapter
+// that occurs among them; only the adapter's own rows are kept. The K blocks of all these products are cut into one
+// stretch per CTA (Cut), the parts are joined by a kernel of their own, which also leaves u as a pair of 16-bit numbers.
+
+// The adapters that occur in a block of 256 rows, in the order of their first rows.
+__global__ void __launch_bounds__(256) lora_list_kernel(const __grid_constant__ LoraArgs g) {
+    __shared__ int ids[256], rank_of[256], count[8];
     griddep_wait();
     griddep_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, quad = lane & 3;
-    if (blockIdx.x == 0 && blockIdx.y == 0) g.arrived[threadIdx.x] = 0;
-    const int m0 = blockIdx.x * 16, r0 = blockIdx.y * 8 * NT;
-    if (threadIdx.x < 16) {
-        const int s = m0 + threadIdx.x < g.M ? __ldca(g.row_adapter + m0 + threadIdx.x) : -1;
-        ids[threadIdx.x] = static_cast<unsigned>(s) < static_cast<unsigned>(g.num_adapters) ? s : -1;
+    const int i = threadIdx.x, m = blockIdx.x * 256 + i, warp = i >> 5, lane = i & 31;
+    const int id = row_adapter(g, m);
+    ids[i] = id;
+    __syncthreads();
+    int first = 0;
+    while (first < i && ids[first] != id) ++first;
+    const uint32_t firsts = __ballot_sync(0xffffffffu, id >= 0 && first == i);
+    if (lane == 0) count[warp] = __popc(firsts);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        before += w < warp ? count[w] : 0;
+        all += count[w];
+    }
+    if (id >= 0 && first == i) {
+        rank_of[i] = before + __popc(firsts & ((1u << lane) - 1u));
+        g.list.adapter[blockIdx.x * 256 + rank_of[i]] = id;
     }
     __syncthreads();
-    const uint16_t *const x0 = g.A + static_cast<int64_t>(m0 + row) * g.K + quad * 8;
-    const bool in0 = m0 + row < g.M, in1 = m0 + row + 8 < g.M;
-    for (int first = 0; first < 16; ++first) {
-        const int s = ids[first];
-        bool seen = s < 0;
-        for (int i = 0; i < first; ++i) seen = seen || ids[i] == s;
-        if (seen) continue;
-        float acc[NT][4] = {};
-        const uint16_t *const a0 = g.lora_a + (static_cast<int64_t>(s) * g.rank + r0 + row) * g.K + quad * 8;
-#pragma unroll 2
-        for (int k = warp * 32; k < g.K; k += 256) {
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const bool in = k + quad * 8 < g.K;
-            const uint4 p = in && in0 ? __ldcg(reinterpret_cast<const uint4 *>(x0 + k)) : zero;
-            const uint4 q = in && in1 ? __ldcg(reinterpret_cast<const uint4 *>(x0 + 8 * static_cast<int64_t>(g.K) + k)) : zero;
-            uint4 b[NT];
+    if (m < g.M) g.list.entry[m] = id >= 0 ? rank_of[first] : -1;
+    if (i == 0) g.list.count[blockIdx.x] = all;
+}
+
+// before[b] = adapters listed in the blocks before block b, before[blocks] = all; one warp.
+__device__ __forceinline__ void scan_lists(const LoraArgs &g, int blocks, int lane, int *before) {
+    int sum = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 32) {
+        int v = b0 + lane < blocks ? __ldcg(g.list.count + b0 + lane) : 0;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                b[t] = in && r0 + 8 * t + row < g.rank ? __ldcg(reinterpret_cast<const uint4 *>(a0 + static_cast<int64_t>(8 * t) * g.K + k)) : zero;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                mma_16816<T>(acc[t], p.x, q.x, p.y, q.y, b[t].x, b[t].y);
-                mma_16816<T>(acc[t], p.z, q.z, p.w, q.w, b[t].z, b[t].w);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        if (b0 + lane < blocks) before[b0 + lane + 1] = sum + v;
+        sum += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) before[0] = 0;
+}
+
+constexpr int kShrinkThreads = 192;                        // TMA, MMA and four draining warps
+constexpr int kShrinkStages = 4;
+constexpr int kShrinkStageBytes = (128 + 256) * 128;
+constexpr int kShrinkSmem = 1024 + kShrinkStages * kShrinkStageBytes + (kMaxBlocks + 1) * 4 + 16 + (2 * kShrinkStages + 4) * 8 + 16;
+
+struct ShrinkWalker {
+    int q, end;
+    Cut cut;
+    __device__ __forceinline__ ShrinkWalker(const Cut &c) : cut(c) {
+        q = static_cast<int>(min(static_cast<long long>(blockIdx.x) * c.len, static_cast<long long>(c.total)));
+        end = min(q + c.len, c.total);
+    }
+    // block of rows, entry of its list, K blocks [kb0, kb1), part
+    __device__ __forceinline__ bool next(const int *before, int blocks, int &block, int &entry, int &kb0, int &kb1, int &part) {
+        if (q >= end) return false;
+        const int unit = q / cut.kblocks;
+        int lo = 0, hi = blocks - 1;                       // the last block whose list does not begin behind the unit
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (before[mid] <= unit) lo = mid;
+            else hi = mid - 1;
+        }
+        block = lo;
+        entry = unit - before[lo];
+        kb0 = q - unit * cut.kblocks;
+        kb1 = min(cut.kblocks, kb0 + end - q);
+        part = static_cast<int>(blockIdx.x) - cut.first_cta(unit);
+        q += kb1 - kb0;
+        return true;
+    }
+};
+
+__global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_kernel(const __grid_constant__ LoraArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t ring = (raw + 1023u) & ~1023u;
+    uint8_t *const sm = smem_raw + (ring - raw);
+    constexpr int kOffBefore = kShrinkStages * kShrinkStageBytes, kOffBars = kOffBefore + ((kMaxBlocks + 1) * 4 + 15) / 16 * 16;
+    int *const before = reinterpret_cast<int *>(sm + kOffBefore);
+    const uint32_t full0 = ring + kOffBars, empty0 = full0 + 8 * kShrinkStages, acc_full0 = empty0 + 8 * kShrinkStages, acc_empty0 = acc_full0 + 16,
+                   misc_at = acc_empty0 + 16;
+    volatile int *const misc = reinterpret_cast<volatile int *>(sm + (misc_at - ring));
+    const WaitCtx wait = {g.status, misc, g.budget};
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    if (tid < 2 * kShrinkStages + 4) {
+        mbar_init(full0 + 8 * tid, tid < 2 * kShrinkStages + 2 ? 1 : 4);
+        fence_mbar_init();
+    }
+    if (tid == 0) misc[0] = 0;
+    if (warp == 1) {
+        tmem_alloc<1>(misc_at + 4, 512);
+        tmem_relinquish<1>();
+    }
+    griddep_wait();
+    const int blocks = (g.M + 255) / 256;
+    if (warp == 0) scan_lists(g, blocks, lane, before);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    griddep_launch_dependents();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[1]), 0);
+    ShrinkWalker walk(Cut(before[blocks], (g.K + 63) / 64, gridDim.x, g.parts_u));
+    int block, entry, kb0, kb1, part, st = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    if (warp == 0) {
+        const bool issuer = elect_one();
+        const uint64_t keep = l2_policy(2);                // A is read again by the product
+        while (ok && walk.next(before, blocks, block, entry, kb0, kb1, part)) {
+            const int row = __ldcg(g.list.adapter + block * 256 + entry) * g.rank;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 3000 + st);
+                if (!ok) break;
+                const uint32_t dst = ring + st * kShrinkStageBytes, bar = full0 + 8 * st;
+                if (issuer) {
+                    mbar_arrive_expect_tx(bar, (g.rank + 256) * 128);
+                    tma_load_2d(dst, &g.map_la, bar, kb * 64, row);
+                    tma_load_2d_hint(dst + 128 * 128, &g.map_a, bar, kb * 64, block * 256, keep);
+                    tma_load_2d_hint(dst + 256 * 128, &g.map_a, bar, kb * 64, block * 256 + 128, keep);
+                }
+                if (++st == kShrinkStages) st = 0, ph ^= 1u;
             }
         }
-        __syncthreads();
+    } else if (warp == 1) {
+        const bool issuer = elect_one();
+        for (int n = 0; ok && walk.next(before, blocks, block, entry, kb0, kb1, part); ++n) {
+            const int acc = n & 1;
+            ok = wait_warp(acc_empty0 + 8 * acc, ((n >> 1) & 1) ^ 1u, wait, 3100 + acc);
+            if (!ok) break;
+            tc_fence_after_sync();
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = wait_warp(full0 + 8 * st, ph, wait, 3200 + st);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t at = ring + st * kShrinkStageBytes;
+                const uint64_t a = umma_desc_sw128(at), x = umma_desc_sw128(at + 128 * 128);
+                if (issuer) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            *reinterpret_cast<float2 *>(&sums[warp][row][8 * t + 2 * quad]) = make_float2(acc[t][0], acc[t][1]);
-            *reinterpret_cast<float2 *>(&sums[warp][row + 8][8 * t + 2 * quad]) = make_float2(acc[t][2], acc[t][3]);
+                    for (int i = 0; i < 4; ++i) umma_f16<1>(tmem + acc * 256, a + 2 * i, x + 2 * i, g.idesc_u, kb > kb0 || i > 0);
+                    umma_commit<1>(empty0 + 8 * st);
+                }
+                if (++st == kShrinkStages) st = 0, ph ^= 1u;
+            }
+            if (ok && issuer) umma_commit<1>(acc_full0 + 8 * acc);
         }
-        __syncthreads();
-        const float scale = g.scale ? g.scale[s] : 1.0f;
-        for (int i = threadIdx.x; i < 16 * 8 * NT; i += 256) {
-            const int m = i / (8 * NT), r = i % (8 * NT);
-            if (ids[m] != s || r0 + r >= g.rank) continue;
-            float v = 0.0f;
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, r = quarter * 32 + lane;   // a rank; ranks from g.rank on are other memory's
+        for (int n = 0; ok && walk.next(before, blocks, block, entry, kb0, kb1, part); ++n) {
+            const int acc = n & 1;
+            ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 3300 + acc);
+            if (!ok) break;
+            tc_fence_after_sync();
+            for (int c = 0; c < 256; c += 32) {
+                const int64_t m = static_cast<int64_t>(block) * 256 + c;
+                const int mine = m + lane < g.M ? __ldcg(g.list.entry + m + lane) : -1;
+                const uint32_t own = __ballot_sync(0xffffffffu, mine == entry);
+                if (own == 0u) continue;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) v += sums[w][m][r];
-            g.u[static_cast<int64_t>(m0 + m) * g.rank + r0 + r] = scale * v;
+                for (int h = 0; h < 32; h += 16) {
+                    uint32_t v[16];
+                    tmem_ld_32x16(tmem + acc * 256 + c + h + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (r < g.rank && (own >> (h + j) & 1u)) g.u_parts[(static_cast<int64_t>(part) * g.M + m + h + j) * g.rank + r] = __uint_as_float(v[j]);
+                    __syncwarp();
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty0 + 8 * acc);
         }
     }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        if (misc[0]) {   // aborted: give copies and MMAs in flight a bounded time to land before the memory goes
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {
+            }
+        }
+        tc_fence_after_sync();
+        tmem_dealloc<1>(tmem, 512);
+    }
+}
+
+// u from its parts, ascending: 32 rows per block, four ranks per thread; as floats and as pairs of 16-bit numbers, and whether the rows' u fit those.
+template <typename T>
+__global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ LoraArgs g) {
+    __shared__ int before[kMaxBlocks + 1];
+    griddep_launch_dependents();   // the product waits for this kernel where it reads u
+    griddep_wait();
+    const int blocks = (g.M + 255) / 256;
+    if (threadIdx.x < 32) scan_lists(g, blocks, threadIdx.x, before);
+    __syncthreads();
+    const Cut cut(before[blocks], (g.K + 63) / 64, g.sms, g.parts_u);
+    const int quads = g.rank / 4;
+    bool fits = true;
+    for (int i = threadIdx.x; i < 32 * quads; i += 256) {
+        const int m = blockIdx.x * 32 + i / quads, r = i % quads * 4;
+        const int entry = m < g.M ? __ldcg(g.list.entry + m) : -1;
+        if (entry < 0) continue;
+        const int parts = cut.num_parts(before[m >> 8] + entry);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const float4 w = __ldcg(reinterpret_cast<const float4 *>(g.u_parts + (static_cast<int64_t>(p) * g.M + m) * g.rank + r));
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+        const float scale = g.scale ? g.scale[g.row_adapter[m]] : 1.0f;
+        const float f[4] = {scale * v.x, scale * v.y, scale * v.z, scale * v.w};
+        *reinterpret_cast<float4 *>(g.u + static_cast<int64_t>(m) * g.rank + r) = make_float4(f[0], f[1], f[2], f[3]);
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            T::split(f[j], hi[j], lo[j]);
+            fits = fits && fabsf(f[j]) <= T::kMax;
+        }
+        *reinterpret_cast<uint2 *>(g.u16 + static_cast<int64_t>(m) * g.rank + r) = make_uint2(hi[0] | static_cast<uint32_t>(hi[1]) << 16, hi[2] | static_cast<uint32_t>(hi[3]) << 16);
+        *reinterpret_cast<uint2 *>(g.u16 + (static_cast<int64_t>(g.M) + m) * g.rank + r) = make_uint2(lo[0] | static_cast<uint32_t>(lo[1]) << 16, lo[2] | static_cast<uint32_t>(lo[3]) << 16);
+    }
+    const int all = __syncthreads_and(fits);
+    if (threadIdx.x == 0) g.list.wide[blockIdx.x] = !all;
 }
 
 // ---------------------------------------------------------------------------------------------- shared product
@@ -222,107 +414,114 @@ struct LoraWalker {
     }
 };
 
-// One column n of D, four rows: sum over the ranks of u[j][r] * lora_b[s[j]][n][r], fp32, two ranks at a time. u lies in shared memory.
-// Where the four rows have one adapter, its ranks are kept as floats from one call to the next (h.w, h.s: whose they
-// are; up to 64 of them): a prompt's rows cost 32 packed multiply-adds each. Else every row's are read, 32 ranks at a
-// time: 16 loads of 16 bytes in flight per lane, which is what reading each adapter once from memory takes.
-struct Held {
-    float2 w[32];
-    int s;
-};
-
+// Rows with adapters of their own: one column n per lane, four rows at a time, fp32 on pairs of ranks. The rows' adapters are read 32
+// ranks at a time: 16 loads of 16 bytes (or 8 of a whole sector) in flight per lane.
 template <typename T>
-__device__ __forceinline__ void adapters_product(const LoraArgs &g, Held &h, const int (&s)[4], const float *u, int n, float (&d)[4]) {
-    const int rank = g.rank;
-    if (s[0] >= 0 && s[0] == s[1] && s[0] == s[2] && s[0] == s[3] && rank <= 64) {
-        if (h.s != s[0]) {
-            const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[0]) * g.N + n) * rank);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint4 v = i * 8 < rank ? __ldcg(b + i) : make_uint4(0, 0, 0, 0);
-                h.w[4 * i] = T::unpack(v.x), h.w[4 * i + 1] = T::unpack(v.y), h.w[4 * i + 2] = T::unpack(v.z), h.w[4 * i + 3] = T::unpack(v.w);
-            }
-            h.s = s[0];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float4 *const uj = reinterpret_cast<const float4 *>(u + j * rank);
-            float2 a = make_float2(0.0f, 0.0f), b = a;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                if (i * 4 >= rank) break;
-                const float4 f = uj[i], e = uj[i + 1];
-                a = fma2(make_float2(f.x, f.y), h.w[2 * i], a);
-                b = fma2(make_float2(f.z, f.w), h.w[2 * i + 1], b);
-                a = fma2(make_float2(e.x, e.y), h.w[2 * i + 2], a);
-                b = fma2(make_float2(e.z, e.w), h.w[2 * i + 3], b);
-            }
-            d[j] = (a.x + a.y) + (b.x + b.y);
-        }
-        return;
-    }
+__device__ __forceinline__ void four_rows(const LoraArgs &g, const int4 id, const float *u, int pitch, int n, float *d) {
+    const int rank = g.rank, s[4] = {id.x, id.y, id.z, id.w};
     const bool wide = g.wide_b != 0;
-    h.s = -1;                                              // its place takes the rows' elements as they were read
     float2 sum[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
     for (int r = 0; r < rank; r += 32) {
+        uint4 b[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint4 *const b = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[j]) * g.N + n) * rank + r);
+            const uint4 *const p = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(s[j]) * g.N + n) * rank + r);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                uint4 v = make_uint4(0, 0, 0, 0), w = v;
+                b[j][i] = b[j][i + 1] = make_uint4(0, 0, 0, 0);
                 if (s[j] >= 0 && r + 8 * i < rank) {
-                    if (wide) ld_32(b + i, v, w);          // a whole sector per lane
+                    if (wide) ld_32(p + i, b[j][i], b[j][i + 1]);
                     else {
-                        v = __ldcg(b + i);
-                        if (r + 8 * i + 8 < rank) w = __ldcg(b + i + 1);
+                        b[j][i] = __ldcg(p + i);
+                        if (r + 8 * i + 8 < rank) b[j][i + 1] = __ldcg(p + i + 1);
                     }
                 }
-                h.w[8 * j + 2 * i] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
-                h.w[8 * j + 2 * i + 1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
-                h.w[8 * j + 2 * i + 2] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
-                h.w[8 * j + 2 * i + 3] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
             }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (s[j] < 0) continue;
-            const float4 *const uj = reinterpret_cast<const float4 *>(u + j * rank + r);
+            const float4 *const uj = reinterpret_cast<const float4 *>(u + j * pitch + r);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (r + 8 * i >= rank) break;
                 const float4 f = uj[2 * i], e = uj[2 * i + 1];
-                sum[j] = fma2(make_float2(f.x, f.y), T::unpack(__float_as_uint(h.w[8 * j + 2 * i].x)), sum[j]);
-                sum[j] = fma2(make_float2(f.z, f.w), T::unpack(__float_as_uint(h.w[8 * j + 2 * i].y)), sum[j]);
-                sum[j] = fma2(make_float2(e.x, e.y), T::unpack(__float_as_uint(h.w[8 * j + 2 * i + 1].x)), sum[j]);
-                sum[j] = fma2(make_float2(e.z, e.w), T::unpack(__float_as_uint(h.w[8 * j + 2 * i + 1].y)), sum[j]);
+                sum[j] = fma2(make_float2(f.x, f.y), T::unpack(b[j][i].x), sum[j]);
+                sum[j] = fma2(make_float2(f.z, f.w), T::unpack(b[j][i].y), sum[j]);
+                sum[j] = fma2(make_float2(e.x, e.y), T::unpack(b[j][i].z), sum[j]);
+                sum[j] = fma2(make_float2(e.z, e.w), T::unpack(b[j][i].w), sum[j]);
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = sum[j].x + sum[j].y;
+    for (int j = 0; j < 4; ++j) d[j * 128] = sum[j].x + sum[j].y;
 }
 
-// The pieces of one CTA's adapters' product in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
+// How the rows of a 256-row tile get their adapters, per group of 32: rows of one adapter whose u fits 16-bit pairs on the tensor core (its
+// zeros would not keep another adapter's infinities out, but these groups have none), other rows with adapters in
+// pieces. One warp; lane i < 8 holds the adapter of group i.
+struct Groups {
+    uint32_t run, piece;
+    int adapter;
+};
+
+__device__ __forceinline__ Groups tile_groups(const LoraArgs &g, int m0, int lane) {
+    Groups v = {0u, 0u, -1};
+    int id[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) id[i] = row_adapter(g, m0 + kGroup * i + lane);
+    const int wide = lane < 8 && m0 + kGroup * lane < g.M ? __ldcg(g.list.wide + m0 / kGroup + lane) : 0;
+    const uint32_t no_run = __ballot_sync(0xffffffffu, wide != 0 || !g.on_tensor);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int first = __shfl_sync(0xffffffffu, id[i], 0);
+        const bool one = __all_sync(0xffffffffu, id[i] == first || id[i] == kNoRow), some = __any_sync(0xffffffffu, id[i] >= 0);
+        if (one && first >= 0 && !(no_run >> i & 1u)) v.run |= 1u << i;
+        else if (some) v.piece |= 1u << i;
+        if (lane == i) v.adapter = first;
+    }
+    return v;
+}
+
+// The next run of groups with one adapter from group `at` on: [from, at), its adapter; false when there is none.
+__device__ __forceinline__ bool next_run(const Groups &v, int &at, int &from, int &adapter) {
+    while (at < 8 && !(v.run >> at & 1u)) ++at;
+    if (at >= 8) return false;
+    from = at;
+    adapter = __shfl_sync(0xffffffffu, v.adapter, at);
+    do {
+        ++at;
+    } while (at < 8 && (v.run >> at & 1u) && __shfl_sync(0xffffffffu, v.adapter, at) == adapter);
+    return true;
+}
+
+// Whether piece c of a tile is one that the delta warps compute for this part of it: with few rows all are, the parts of a tile share them.
+template <bool WAVES>
+__device__ __forceinline__ bool has_piece(const LoraSegment &s, const Groups &v, int c) {
+    return WAVES ? (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u : c % s.parts == s.part;
+}
+
+// The pieces of one CTA in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
 template <int CG, bool WAVES>
 struct PieceWalker {
     LoraWalker<CG, WAVES> walk;
     LoraSegment s;
+    Groups v;
     int c, rows;
-    __device__ __forceinline__ PieceWalker(const LoraWalker<CG, WAVES> &w) : walk(w) {
-        c = rows = 0;
-        s.parts = 0;
-    }
-    __device__ __forceinline__ bool next(const LoraArgs &g) {
-        c += s.parts;
-        while (c * kChunkRows >= rows) {
-            if (!walk.next(s)) return false;
-            rows = min(g.rows, g.M - s.m0);
-            c = s.part;
+    __device__ __forceinline__ PieceWalker(const LoraWalker<CG, WAVES> &w) : walk(w) { c = rows = 0; }
+    __device__ __forceinline__ bool next(const LoraArgs &g, int lane) {
+        ++c;
+        for (;; ++c) {
+            while (c * kChunkRows >= rows) {
+                if (!walk.next(s)) return false;
+                if (WAVES) v = tile_groups(g, s.m0, lane);
+                rows = min(g.rows, g.M - s.m0);
+                c = 0;
+            }
+            if (has_piece<WAVES>(s, v, c)) return true;
         }
-        return true;
     }
 };
 
@@ -336,8 +535,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     float *const u_s = reinterpret_cast<float *>(sm + g.off_u);
     int *const id_s = reinterpret_cast<int *>(sm + g.off_ids);
     const uint32_t full0 = ring + g.off_bars, empty0 = full0 + 8 * kLoraStages, acc_full0 = empty0 + 8 * kLoraStages, acc_empty0 = acc_full0 + 16,
-                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kChunks,
-                   u_full0 = delta_empty0 + 8 * kChunks, u_empty0 = u_full0 + 8 * kAhead;
+                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kMaxChunks,
+                   u_full0 = delta_empty0 + 8 * kMaxChunks, u_empty0 = u_full0 + 8 * kAhead;
     volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // abort flag, tensor-memory base, two tiles whose parts this CTA adds
     const WaitCtx wait = {g.status, misc, g.budget};
     const int tid = threadIdx.x, lane = tid & 31;
@@ -346,8 +545,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
 
     if (tid < kLoraBars) {
         // accumulators: full, empty (the draining warps of the pair); pieces: full (the delta warps), empty (the draining warps); u: full, empty
-        const int j = tid - 2 * kLoraStages, i = j - 4 - 2 * kChunks;
-        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kChunks ? kDeltaWarps : i < 0 ? 4 : i < kAhead ? 1 : kDeltaWarps);
+        const int j = tid - 2 * kLoraStages, i = j - 4 - 2 * kMaxChunks;
+        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kMaxChunks ? kDeltaWarps : i < 0 ? 4 : i < kAhead ? 1 : kDeltaWarps);
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0, misc[2] = misc[3] = -1;
@@ -403,6 +602,26 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 }
                 if (++st == stages) st = 0, ph ^= 1u;
             }
+            if constexpr (WAVES) {
+                // then the adapters of whole groups: 64 ranks of lora_b and of u's values, the same ranks and u's remainders
+                griddep_wait();
+                const Groups v = tile_groups(g, s.m0, lane);
+                int at = 0, from, adapter;
+                while (ok && next_run(v, at, from, adapter)) {
+                    const int row_u = s.m0 + kGroup * from + static_cast<int>(rank) * (kGroup * (at - from) / 2);
+                    for (int i = 0; i < (g.rank + 63) / 64 * 2; ++i) {
+                        ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 2000 + st);
+                        if (!ok) break;
+                        const uint32_t dst = ring + st * stage_bytes;
+                        if (issuer) {
+                            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * st, CG * stage_bytes);
+                            tma_load_2d_pair(dst, &g.map_lb, full_leader + 8 * st, (i >> 1) * 64, adapter * g.N + row_b);
+                            tma_load_2d_pair(dst + kBBytes, &g.map_u, full_leader + 8 * st, (i >> 1) * 64, (i & 1) * g.M + row_u);
+                        }
+                        if (++st == stages) st = 0, ph ^= 1u;
+                    }
+                }
+            }
         }
     } else if (warp == 1) {
         // -------------------------------------------------------------- MMA
@@ -427,6 +646,27 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                     }
                     if (++st == stages) st = 0, ph ^= 1u;
                 }
+                if constexpr (WAVES) {
+                    griddep_wait();
+                    const Groups v = tile_groups(g, s.m0, lane);
+                    int at = 0, from, adapter;
+                    while (ok && next_run(v, at, from, adapter)) {
+                        const uint32_t idesc = g.idesc_run | static_cast<uint32_t>(kGroup * (at - from) / 8) << 17;
+                        for (int i = 0; i < (g.rank + 63) / 64 * 2; ++i) {
+                            ok = wait_warp(full0 + 8 * st, ph, wait, 2200 + st);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+                            const uint32_t stage = ring + st * stage_bytes;
+                            const uint64_t b = umma_desc_sw128(stage), a = umma_desc_sw128(stage + kBBytes);
+                            const int steps = min(4, (g.rank - (i >> 1) * 64 + 15) / 16);
+                            if (issuer) {
+                                for (int j = 0; j < steps; ++j) umma_f16<CG>(d + kGroup * from, b + 2 * j, a + 2 * j, idesc, 1);
+                                commit_cta<CG>(empty0 + 8 * st);
+                            }
+                            if (++st == stages) st = 0, ph ^= 1u;
+                        }
+                    }
+                }
                 if (ok && issuer) commit_cta<CG>(acc_full0 + 8 * acc);
             }
         }
@@ -435,29 +675,32 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         // -------------------------------------------------------------- accumulators (+ the adapters' product) -> D or parts
         const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t acc_empty_leader = CG == 2 ? mapa_shared(acc_empty0, 0) : acc_empty0;
-        int piece = 0;
+        int slot = 0;
+        uint32_t slot_ph = 0;
         griddep_wait();                                    // the counters below are zero
         for (int n = 0; ok && walk.next(s); ++n) {
             const int acc = n & 1, rows = min(g.rows, g.M - s.m0);
             const int col = (s.tile * CG + static_cast<int>(rank)) * 128 + r;
             const bool mine = col < g.N;
+            Groups v_groups = {};
+            if (WAVES) v_groups = tile_groups(g, s.m0, lane);
             ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 2300 + acc);
             if (!ok) break;
             tc_fence_after_sync();
             for (int c = 0; c * kChunkRows < rows; ++c) {
-                uint32_t v[8];
-                tmem_ld_32x8(tmem + acc * g.rows + c * kChunkRows + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                uint32_t v[16];
+                tmem_ld_32x16(tmem + acc * g.rows + c * kChunkRows + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                const bool add = has_piece<WAVES>(s, v_groups, c);
+                if (add) ok = wait_warp(delta_full0 + 8 * slot, slot_ph, wait, 2400 + slot);
                 tmem_ld_wait();
-                if (c % s.parts == s.part) {               // the parts of a tile share its pieces
-                    const int slot = piece % kChunks;
-                    ok = wait_warp(delta_full0 + 8 * slot, (piece / kChunks) & 1, wait, 2400 + slot);
-                    if (!ok) break;
+                if (!ok) break;
+                if (add) {
 #pragma unroll
                     for (int j = 0; j < kChunkRows; ++j)
                         v[j] = __float_as_uint(__uint_as_float(v[j]) + delta[(slot * kChunkRows + j) * 128 + r]);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(delta_empty0 + 8 * slot);
-                    ++piece;
+                    if (++slot == g.chunks) slot = 0, slot_ph ^= 1u;
                 }
                 if (mine) {
                     const int64_t row = s.m0 + c * kChunkRows;
@@ -495,47 +738,58 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         }
     } else if (warp < 6 + kDeltaWarps) {
         // -------------------------------------------------------------- the adapters' product
-        const int t = tid - 6 * 32, n = t & 127, half = (t >> 7) * 4;
-        Held held;
-        held.s = -1;
-        int held_col = -1;
+        const int w = warp - 6, n = (w & 3) * 32 + lane, half = (w >> 2) * 8;
+        int slot = 0, from = 0;
+        uint32_t slot_ph = 1, from_ph = 0;
         PieceWalker<CG, WAVES> at(walk);
         griddep_wait();                                    // nothing that this SM's first-level cache may hold is older than the operands
-        for (int piece = 0; ok && at.next(g); ++piece) {
-            const int slot = piece % kChunks, from = piece % kAhead, col = (at.s.tile * CG + static_cast<int>(rank)) * 128 + n;
-            if (col != held_col) held.s = -1, held_col = col;
-            ok = wait_warp(u_full0 + 8 * from, (piece / kAhead) & 1, wait, 2600 + from);
+        while (ok && at.next(g, lane)) {
+            const int col0 = (at.s.tile * CG + static_cast<int>(rank)) * 128;
+            ok = wait_warp(u_full0 + 8 * from, from_ph, wait, 2600 + from);
             if (!ok) break;
-            const int4 q = *reinterpret_cast<const int4 *>(id_s + from * kChunkRows + half);
-            const int id[4] = {q.x, q.y, q.z, q.w};
-            float d[4] = {};
-            if (col < g.N) adapters_product<T>(g, held, id, u_s + (from * kChunkRows + half) * g.rank, col, d);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(u_empty0 + 8 * from);
-            ok = wait_warp(delta_empty0 + 8 * slot, ((piece / kChunks) & 1) ^ 1u, wait, 2500 + slot);
+            const int *const id = id_s + from * kChunkRows;
+            const float *const u = u_s + from * kChunkRows * g.u_pitch;
+            float *const d = delta + slot * kChunkRows * 128;
+            ok = wait_warp(delta_empty0 + 8 * slot, slot_ph, wait, 2500 + slot);
             if (!ok) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) delta[(slot * kChunkRows + half + j) * 128 + n] = d[j];
+            if (col0 + n < g.N) {
+#pragma unroll 1
+                for (int j = half; j < half + 8; j += 4)
+                    four_rows<T>(g, *reinterpret_cast<const int4 *>(id + j), u + j * g.u_pitch, g.u_pitch, col0 + n, d + j * 128 + n);
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(delta_full0 + 8 * slot);
+            if (lane == 0) {
+                mbar_arrive(u_empty0 + 8 * from);
+                mbar_arrive(delta_full0 + 8 * slot);
+            }
+            if (++from == kAhead) from = 0, from_ph ^= 1u;
+            if (++slot == g.chunks) slot = 0, slot_ph ^= 1u;
         }
     } else {
         // -------------------------------------------------------------- u and the rows' adapters for the warps above
         PieceWalker<CG, WAVES> at(walk);
+        int from = 0;
+        uint32_t ph_from = 1;
         griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
-        for (int piece = 0; ok && at.next(g); ++piece) {
-            const int from = piece % kAhead, m = at.s.m0 + at.c * kChunkRows;
-            int id = -1;
-            if (lane < kChunkRows && m + lane < g.M) id = __ldca(g.row_adapter + m + lane);
-            ok = wait_warp(u_empty0 + 8 * from, ((piece / kAhead) & 1) ^ 1u, wait, 2700 + from);
-            if (!ok) break;
-            if (lane < kChunkRows) id_s[from * kChunkRows + lane] = static_cast<unsigned>(id) < static_cast<unsigned>(g.num_adapters) ? id : -1;
-            __syncwarp();
-            if (lane == 0) {
-                const uint32_t bytes = static_cast<uint32_t>(min(kChunkRows, g.M - m) * g.rank * 4);
-                mbar_arrive_expect_tx(u_full0 + 8 * from, bytes);
-                bulk_load(smem_u32(u_s + from * kChunkRows * g.rank), g.u + static_cast<int64_t>(m) * g.rank, bytes, u_full0 + 8 * from);
+        while (ok && at.next(g, lane)) {
+            const int m = at.s.m0 + at.c * kChunkRows + lane;
+            const bool there = lane < kChunkRows && m < g.M;
+            const int id = lane < kChunkRows ? row_adapter(g, m) : kNoRow;
+            if (id >= 0) {
+                // what the piece will read of the adapter: 128 of its columns, which lie behind one another
+                const int col = (at.s.tile * CG + static_cast<int>(rank)) * 128;
+                if (col < g.N) prefetch_l2(g.lora_b + (static_cast<int64_t>(id) * g.N + col) * g.rank, static_cast<uint32_t>(min(128, g.N - col) * g.rank * 2));
             }
+            ok = wait_warp(u_empty0 + 8 * from, ph_from, wait, 2700 + from);
+            if (!ok) break;
+            const int rows = __popc(__ballot_sync(0xffffffffu, there));
+            if (lane < kChunkRows) id_s[from * kChunkRows + lane] = id;
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(u_full0 + 8 * from, static_cast<uint32_t>(rows * g.rank * 4));
+            __syncwarp();
+            if (there)
+                bulk_load(smem_u32(u_s + (from * kChunkRows + lane) * g.u_pitch), g.u + static_cast<int64_t>(m) * g.rank, static_cast<uint32_t>(g.rank * 4), u_full0 + 8 * from);
+            if (++from == kAhead) from = 0, ph_from ^= 1u;
         }
     }
 
@@ -552,16 +806,27 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             const int parts = walk.cut.num_parts(tile), col = (tile * CG + static_cast<int>(rank)) * 128 + lane * 4;
             if (col >= g.N) continue;
             const int64_t pitch = static_cast<int64_t>(g.M) * g.N;
-            for (int m = warp; m < g.M; m += kLoraThreads / 32) {
-                const float *o = g.o + static_cast<int64_t>(m) * g.N + col;
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                for (int p = 0; p < parts; ++p) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(o + p * pitch));
-                    y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+            constexpr int kWarps = kLoraThreads / 32;
+            for (int m = warp; m < g.M; m += 2 * kWarps) {  // two rows and four parts of each in flight
+                const float *const o = g.o + static_cast<int64_t>(m) * g.N + col, *const o2 = o + static_cast<int64_t>(kWarps) * g.N;
+                const bool two = m + kWarps < g.M;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y2 = y;
+                for (int p0 = 0; p0 < parts; p0 += 4) {
+                    float4 v[4], v2[4];
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        v[p] = v2[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (p0 + p < parts) v[p] = __ldcg(reinterpret_cast<const float4 *>(o + (p0 + p) * pitch));
+                        if (p0 + p < parts && two) v2[p] = __ldcg(reinterpret_cast<const float4 *>(o2 + (p0 + p) * pitch));
+                    }
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        y.x += v[p].x, y.y += v[p].y, y.z += v[p].z, y.w += v[p].w;
+                        y2.x += v2[p].x, y2.y += v2[p].y, y2.z += v2[p].z, y2.w += v2[p].w;
+                    }
                 }
-                *reinterpret_cast<uint2 *>(g.D + static_cast<int64_t>(m) * g.N + col) =
-                    make_uint2(T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16, T::round(y.z) | static_cast<uint32_t>(T::round(y.w)) << 16);
+                store_four<T>(g.D + static_cast<int64_t>(m) * g.N + col, y);
+                if (two) store_four<T>(g.D + static_cast<int64_t>(m + kWarps) * g.N + col, y2);
             }
         }
     }
@@ -597,13 +862,13 @@ cudaError_t launch(Kernel *kernel, const LoraArgs &g, dim3 grid, int threads, in
 template <typename T>
 cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
     cudaError_t e;
-    if (g.M <= kDotRows) {
+    if (g.M <= kFewRows) {
         const int blocks = g.M * (g.rank / 4);
         e = launch(lora_shrink_dot_kernel<T>, g, blocks < 8 * g.sms ? blocks : 8 * g.sms, 256, 0, 1, stream);
     } else {
-        const int row_blocks = (g.M + 15) / 16;
-        if (row_blocks * ((g.rank + 31) / 32) >= g.sms) e = launch(lora_shrink_mma_kernel<T, 4>, g, dim3(row_blocks, (g.rank + 31) / 32), 256, 0, 1, stream);
-        else e = launch(lora_shrink_mma_kernel<T, 1>, g, dim3(row_blocks, g.rank / 8), 256, 0, 1, stream);
+        e = launch(lora_list_kernel, g, (g.M + 255) / 256, 256, 0, 1, stream);
+        if (e == cudaSuccess) e = launch(lora_shrink_kernel, g, g.sms, kShrinkThreads, kShrinkSmem, 1, stream);
+        if (e == cudaSuccess) e = launch(lora_join_kernel<T>, g, (g.M + 31) / 32, 256, 0, 1, stream);
     }
     if (e != cudaSuccess) return e;
     if (g.M <= kOneCtaRows) return launch(lora_product_kernel<T, 1, false>, g, g.sms, kLoraThreads, smem, 1, stream);
@@ -619,22 +884,42 @@ int most_parts(int64_t units, int64_t kblocks, int64_t groups) {
 }
 
 struct LoraLayout {
-    int parts;
-    int64_t off_u, off_o, bytes;
+    int parts, parts_u;
+    int64_t off_u, off_o, off_u16, off_u_parts, off_count, off_adapter, off_entry, off_wide, bytes;
 };
 
 LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int rank) {
-    LoraLayout l;
-    l.parts = M > kFewRows ? 2 : M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
-    l.off_u = kMaxCtas * 4;
-    l.off_o = l.off_u + (M * rank * 4 + 255) / 256 * 256;
-    l.bytes = l.off_o + (M <= kFewRows ? l.parts * M * N * 4 : 0);
+    LoraLayout l = {};
+    if (M > kMaxBlocks * 256) M = kMaxBlocks * 256;
+    int64_t at = 0;
+    auto take = [&at](int64_t bytes) {
+        const int64_t from = at;
+        at += (bytes + 255) / 256 * 256;
+        return from;
+    };
+    take(kMaxCtas * 4);
+    l.off_u = take(M * rank * 4);
+    if (M <= kFewRows) {
+        l.parts = M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
+        l.off_o = take(l.parts * M * N * 4);
+    } else {
+        const int64_t blocks = (M + 255) / 256;
+        l.parts = 2;
+        l.parts_u = most_parts(blocks, (K + 63) / 64, kLoraGridSms);
+        l.off_u16 = take(2 * M * rank * 2);
+        l.off_u_parts = take(l.parts_u * M * rank * 4);
+        l.off_count = take(blocks * 4);
+        l.off_adapter = take(blocks * 256 * 4);
+        l.off_entry = take(M * 4);
+        l.off_wide = take((M + 31) / 32 * 4);
+    }
+    l.bytes = at;
     return l;
 }
 
 int check_lora(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) {
     if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 8) return B200_INVALID_SHAPE;
-    if (M > (int64_t(1) << 22) || N > (int64_t(1) << 30) || K > (int64_t(1) << 30)) return B200_INVALID_SHAPE;
+    if (M > (int64_t(1) << 24) || N > (int64_t(1) << 22) || K > (int64_t(1) << 18)) return B200_INVALID_SHAPE;   // K blocks are counted in 32 bits
     if (num_adapters < 1 || num_adapters > (int64_t(1) << 20)) return B200_INVALID_SHAPE;
     if (rank < 8 || rank > B200_LORA_MAX_RANK || rank % 8) return B200_INVALID_CONFIG;
     return B200_OK;
@@ -650,13 +935,8 @@ int prepare_routed_kernels() {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
     }
-    // An SM that runs the shrink kernel with little shared memory could not take a block of the product beside it.
-    void (*const first[])(LoraArgs) = {lora_shrink_dot_kernel<Bf16>, lora_shrink_mma_kernel<Bf16, 1>, lora_shrink_mma_kernel<Bf16, 4>,
-                                       lora_shrink_dot_kernel<Fp16>, lora_shrink_mma_kernel<Fp16, 1>, lora_shrink_mma_kernel<Fp16, 4>};
-    for (const auto k : first) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        if (e != cudaSuccess) return static_cast<int>(e);
-    }
+    const cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    if (e != cudaSuccess) return static_cast<int>(e);
     return prepare_moe_kernels();
 }
 
@@ -690,44 +970,64 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     if (st != B200_OK) return st;
     if (g.sms > kMaxCtas) g.sms = kMaxCtas;
     const LoraLayout l = lora_layout(M, N, K, rank);
-    g.A = static_cast<const uint16_t *>(A);
     g.lora_a = static_cast<const uint16_t *>(lora_a);
     g.lora_b = static_cast<const uint16_t *>(lora_b);
-    g.D = static_cast<uint16_t *>(D);
     g.scale = lora_scale;
-    g.row_adapter = row_adapter;
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     g.arrived = reinterpret_cast<int *>(ws);
     g.u = reinterpret_cast<float *>(ws + l.off_u);
     g.o = reinterpret_cast<float *>(ws + l.off_o);
-    g.M = static_cast<int>(M);
+    g.u16 = reinterpret_cast<uint16_t *>(ws + l.off_u16);
+    g.u_parts = reinterpret_cast<float *>(ws + l.off_u_parts);
+    g.list.count = reinterpret_cast<int *>(ws + l.off_count);
+    g.list.adapter = reinterpret_cast<int *>(ws + l.off_adapter);
+    g.list.entry = reinterpret_cast<int *>(ws + l.off_entry);
+    g.list.wide = reinterpret_cast<int *>(ws + l.off_wide);
     g.N = static_cast<int>(N);
     g.K = static_cast<int>(K);
     g.rank = rank;
     g.num_adapters = static_cast<int>(num_adapters);
     g.parts = l.parts;
+    g.parts_u = l.parts_u;
+    const bool bf16 = dtype == B200_BF16;
     const int cg = M > kOneCtaRows ? 2 : 1;
     g.rows = M > kFewRows ? 256 : static_cast<int>((M + 16 * cg - 1) / (16 * cg) * (16 * cg));
     const int box_a = g.rows / cg;
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
-    st = encode_operand_map(&g.map_b, dtype, Bt, K, N, 128);
-    if (st == B200_OK) st = encode_operand_map(&g.map_a, dtype, A, K, M, box_a);
-    if (st != B200_OK) return st;
     g.a_bytes = box_a * 128;
-    const int u_bytes = kAhead * kChunkRows * rank * 4, rest = kChunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
-    // up to 256 rows 32 KB of the SM stay free for blocks of the shrink kernel
+    g.u_pitch = rank + 4;   // rows of u start 16 bytes further each, modulo the banks
+    g.chunks = M > 128 || rank > 64 ? 4 : kMaxChunks;
+    const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, rest = g.chunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
     g.stages = ((M > kFewRows ? kSmemLimit : 196 * 1024) - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
-    g.off_u = g.off_delta + kChunks * kChunkBytes;
+    g.off_u = g.off_delta + g.chunks * kChunkBytes;
     g.off_ids = g.off_u + u_bytes;
     g.off_bars = g.off_ids + kAhead * kChunkRows * 4;
     g.off_misc = g.off_bars + kLoraBars * 8;
-    const int smem = 1024 + g.off_delta + rest;
+    const int bytes = 1024 + g.off_delta + rest, smem = bytes < kMinSmemRequest ? kMinSmemRequest : bytes;
     g.tmem_cols = pow2_at_least(2 * g.rows);
-    g.idesc = umma_idesc(128 * cg, g.rows, dtype == B200_BF16);
+    g.idesc = umma_idesc(128 * cg, g.rows, bf16);
+    g.idesc_run = umma_idesc(256, 0, bf16);
+    g.idesc_u = umma_idesc(128, 256, bf16);
     g.budget = wait_budget_cycles();
-    const cudaError_t e = dtype == B200_BF16 ? launch_lora<Bf16>(g, smem < kMinSmemRequest ? kMinSmemRequest : smem, static_cast<cudaStream_t>(stream))
-                                             : launch_lora<Fp16>(g, smem < kMinSmemRequest ? kMinSmemRequest : smem, static_cast<cudaStream_t>(stream));
-    return e != cudaSuccess ? record_cuda_error(e) : B200_OK;
+    st = encode_operand_map(&g.map_b, dtype, Bt, K, N, 128);
+    if (st == B200_OK && M > kFewRows) {
+        g.on_tensor = num_adapters * N < (int64_t(1) << 31) - 512;   // rows of lora_b as the copies count them
+        st = encode_operand_map(&g.map_la, dtype, lora_a, K, num_adapters * rank, rank);
+        if (st == B200_OK && g.on_tensor) st = encode_operand_map(&g.map_lb, dtype, lora_b, rank, num_adapters * N, 128);
+    }
+    for (int64_t m0 = 0; st == B200_OK && m0 < M; m0 += kMaxBlocks * 256) {
+        const int64_t rows = M - m0 < kMaxBlocks * 256 ? M - m0 : kMaxBlocks * 256;
+        g.A = static_cast<const uint16_t *>(A) + m0 * K;
+        g.D = static_cast<uint16_t *>(D) + m0 * N;
+        g.row_adapter = row_adapter + m0;
+        g.M = static_cast<int>(rows);
+        st = encode_operand_map(&g.map_a, dtype, g.A, K, rows, box_a);
+        if (st == B200_OK && M > kFewRows && g.on_tensor) st = encode_operand_map(&g.map_u, dtype, g.u16, rank, 2 * rows, 128);
+        if (st != B200_OK) break;
+        const cudaError_t e = bf16 ? launch_lora<Bf16>(g, smem, static_cast<cudaStream_t>(stream)) : launch_lora<Fp16>(g, smem, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) st = record_cuda_error(e);
+    }
+    return st;
 }

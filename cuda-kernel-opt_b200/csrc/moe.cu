@@ -341,8 +341,7 @@ __device__ __forceinline__ void combine(const MoeArgs &g, int2 *entry, int t, in
                 y.x = fmaf(f, v[i].x, y.x), y.y = fmaf(f, v[i].y, y.y), y.z = fmaf(f, v[i].z, y.z), y.w = fmaf(f, v[i].w, y.w);
             }
     }
-    *reinterpret_cast<uint2 *>(g.Y + static_cast<int64_t>(t) * g.hidden + n) =
-        make_uint2(T::round(y.x) | static_cast<uint32_t>(T::round(y.y)) << 16, T::round(y.z) | static_cast<uint32_t>(T::round(y.w)) << 16);
+    store_four<T>(g.Y + static_cast<int64_t>(t) * g.hidden + n, y);
 }
 
 template <typename T, Product P>

@@ -13,6 +13,7 @@ namespace b200 {
 
 struct Bf16 {
     static constexpr int kCode = B200_BF16;
+    static constexpr float kMax = 3.38953139e38f;
     // two packed elements -> two floats; element 0 sits in the low half
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -21,19 +22,20 @@ struct Bf16 {
     // v as the sum of two elements. The first one saturates, so that infinities (and what the pair cannot hold) arrive as
     // an infinity in the second one, not as infinity minus infinity.
     __device__ static __forceinline__ void split(float v, uint16_t &hi, uint16_t &lo) {
-        hi = round(fminf(fmaxf(v, -3.38953139e38f), 3.38953139e38f));
+        hi = round(fminf(fmaxf(v, -kMax), kMax));
         lo = round(v - __uint_as_float(static_cast<uint32_t>(hi) << 16));
     }
 };
 
 struct Fp16 {
     static constexpr int kCode = B200_F16;
+    static constexpr float kMax = 65504.0f;
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return __half22float2(*reinterpret_cast<const __half2 *>(&v));
     }
     __device__ static __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
     __device__ static __forceinline__ void split(float v, uint16_t &hi, uint16_t &lo) {
-        hi = round(fminf(fmaxf(v, -65504.0f), 65504.0f));
+        hi = round(fminf(fmaxf(v, -kMax), kMax));
         lo = round(v - __half2float(__ushort_as_half(hi)));
     }
 };
@@ -60,24 +62,16 @@ __device__ __forceinline__ float2 fma2(const float2 &a, const float2 &b, const f
     return r;
 }
 
-// acc (16 x 8, fp32) += A (16 x 16) * B (16 x 8); lane = 4 * row + quad holds rows row and row + 8 of A, column row of B
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&acc)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (T::kCode == B200_BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(acc[0]), "+f"(acc[1]), "+f"(acc[2]), "+f"(acc[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(acc[0]), "+f"(acc[1]), "+f"(acc[2]), "+f"(acc[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // 32 bytes at a 32-byte aligned address
 __device__ __forceinline__ void ld_32(const void *p, uint4 &a, uint4 &b) {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
                  : "l"(p));
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(uint16_t *p, const float4 &v) {   // 8-byte aligned
+    *reinterpret_cast<uint2 *>(p) = make_uint2(T::round(v.x) | static_cast<uint32_t>(T::round(v.y)) << 16, T::round(v.z) | static_cast<uint32_t>(T::round(v.w)) << 16);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

@@ -302,7 +302,7 @@ int b200_session_gemm_host_sharded(b200_session *s, int dtype, const void *hA_ro
  * outside [0, num_adapters) has no adapter. Any order of the entries is allowed; rows of one request
  * behind one another share their adapter's reads. Adapters of several ranks are stacked at the largest, filled up
  * with zeros; weights of adapters that no row names are not read. N, K and rank are multiples of 8,
- * rank <= B200_LORA_MAX_RANK. A null row_adapter is refused; num_adapters = 0 is refused (that is b200_gemm_bf16). */
+ * rank <= B200_LORA_MAX_RANK, M <= 2^24, N <= 2^22, K <= 2^18, num_adapters <= 2^20. A null row_adapter is refused; num_adapters = 0 is refused (that is b200_gemm_bf16). */
 enum { B200_LORA_MAX_RANK = 128 };
 int64_t b200_gemm_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank);
 int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D, int64_t M, int64_t N, int64_t K, const void *lora_a,
@@ -320,7 +320,7 @@ int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D, int64_t M,
  * -infinity or NaN is never chosen; where fewer than top_k are left, the other entries of ids are -1 with weight 0, and a
  * token with none gets a zero row; +infinity counts as the largest finite value. ids (int) and weights (float), both
  * tokens x top_k in descending order of the logits, are outputs; either may be null. Weights of experts that no
- * token chose are not read. hidden and inner are multiples of 8, experts <= B200_MOE_MAX_EXPERTS, top_k <=
+ * token chose are not read. hidden and inner are multiples of 8, at most 65536, experts <= B200_MOE_MAX_EXPERTS, top_k <=
  * min(experts, B200_MOE_MAX_TOP_K). */
 enum { B200_MOE_MAX_TOKENS = 256, B200_MOE_MAX_EXPERTS = 512, B200_MOE_MAX_TOP_K = 16 };
 int64_t b200_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k);
