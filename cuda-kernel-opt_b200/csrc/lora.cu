@@ -136,29 +136,42 @@ __global__ void __launch_bounds__(256) lora_shrink_dot_kernel(const __grid_const
 
 // The adapters that occur in a block of 256 rows, in the order of their first rows.
 __global__ void __launch_bounds__(256) lora_list_kernel(const __grid_constant__ LoraArgs g) {
-    __shared__ int ids[256], rank_of[256], count[8];
+    __shared__ int lead_id[8][32], lead_row[8][32], leads[8], rank_of[256], firsts[8];
     griddep_wait();
     griddep_launch_dependents();
     const int i = threadIdx.x, m = blockIdx.x * 256 + i, warp = i >> 5, lane = i & 31;
     const int id = row_adapter(g, m);
-    ids[i] = id;
+    // one row of the warp per adapter leads; it looks for its adapter among the leaders of the warps before
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    const int leader = __ffs(same) - 1;
+    const uint32_t lead = __ballot_sync(0xffffffffu, id >= 0 && leader == lane);
+    if (lead >> lane & 1u) {
+        const int at = __popc(lead & ((1u << lane) - 1u));
+        lead_id[warp][at] = id;
+        lead_row[warp][at] = i;
+    }
+    if (lane == 0) leads[warp] = __popc(lead);
     __syncthreads();
-    int first = 0;
-    while (first < i && ids[first] != id) ++first;
-    const uint32_t firsts = __ballot_sync(0xffffffffu, id >= 0 && first == i);
-    if (lane == 0) count[warp] = __popc(firsts);
+    int first = i;
+    if (lead >> lane & 1u)
+        for (int w = 0; w < warp && first == i; ++w)
+            for (int j = 0; j < leads[w] && first == i; ++j)
+                if (lead_id[w][j] == id) first = lead_row[w][j];
+    const uint32_t new_ones = __ballot_sync(0xffffffffu, (lead >> lane & 1u) && first == i);
+    if (lane == 0) firsts[warp] = __popc(new_ones);
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-        before += w < warp ? count[w] : 0;
-        all += count[w];
+        before += w < warp ? firsts[w] : 0;
+        all += firsts[w];
     }
-    if (id >= 0 && first == i) {
-        rank_of[i] = before + __popc(firsts & ((1u << lane) - 1u));
+    if (new_ones >> lane & 1u) {
+        rank_of[i] = before + __popc(new_ones & ((1u << lane) - 1u));
         g.list.adapter[blockIdx.x * 256 + rank_of[i]] = id;
     }
     __syncthreads();
+    first = __shfl_sync(0xffffffffu, first, leader);
     if (m < g.M) g.list.entry[m] = id >= 0 ? rank_of[first] : -1;
     if (i == 0) g.list.count[blockIdx.x] = all;
 }
@@ -290,24 +303,28 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_kernel(const __
         const int quarter = warp & 3, r = quarter * 32 + lane;   // a rank; ranks from g.rank on are other memory's
         for (int n = 0; ok && walk.next(before, blocks, block, entry, kb0, kb1, part); ++n) {
             const int acc = n & 1;
+            uint32_t own = 0u;                             // lane i < 8: which rows of the i-th 32 have this adapter
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int m = block * 256 + 32 * i + lane;
+                const uint32_t bits = __ballot_sync(0xffffffffu, m < g.M && __ldcg(g.list.entry + m) == entry);
+                if (lane == i) own = bits;
+            }
             ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 3300 + acc);
             if (!ok) break;
             tc_fence_after_sync();
-            for (int c = 0; c < 256; c += 32) {
-                const int64_t m = static_cast<int64_t>(block) * 256 + c;
-                const int mine = m + lane < g.M ? __ldcg(g.list.entry + m + lane) : -1;
-                const uint32_t own = __ballot_sync(0xffffffffu, mine == entry);
-                if (own == 0u) continue;
+#pragma unroll 1
+            for (int c = 0; c < 256; c += 16) {
+                const uint32_t bits = __shfl_sync(0xffffffffu, own, c >> 5) >> (c & 16);
+                if ((bits & 0xffffu) == 0u) continue;
+                uint32_t v[16];
+                tmem_ld_32x16(tmem + acc * 256 + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                tmem_ld_wait();
+                float *const out = g.u_parts + (static_cast<int64_t>(part) * g.M + block * 256 + c) * g.rank + r;
 #pragma unroll
-                for (int h = 0; h < 32; h += 16) {
-                    uint32_t v[16];
-                    tmem_ld_32x16(tmem + acc * 256 + c + h + (static_cast<uint32_t>(quarter * 32) << 16), v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (r < g.rank && (own >> (h + j) & 1u)) g.u_parts[(static_cast<int64_t>(part) * g.M + m + h + j) * g.rank + r] = __uint_as_float(v[j]);
-                    __syncwarp();
-                }
+                for (int j = 0; j < 16; ++j)
+                    if (r < g.rank && (bits >> j & 1u)) out[j * g.rank] = __uint_as_float(v[j]);
+                __syncwarp();
             }
             tc_fence_before_sync();
             __syncwarp();
@@ -327,38 +344,41 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_kernel(const __
     }
 }
 
-// u from its parts, ascending: 32 rows per block, four ranks per thread; as floats and as pairs of 16-bit numbers, and whether the rows' u fit those.
+// u from its parts, ascending: 32 rows per block, four ranks of one row per thread; as floats and as pairs of 16-bit numbers, and whether the
+// rows' u fit those.
 template <typename T>
-__global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ LoraArgs g) {
+__global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__ LoraArgs g) {
     __shared__ int before[kMaxBlocks + 1];
     griddep_launch_dependents();   // the product waits for this kernel where it reads u
     griddep_wait();
-    const int blocks = (g.M + 255) / 256;
+    const int blocks = (g.M + 255) / 256, quads = g.rank / 4;
+    const int m = blockIdx.x * 32 + threadIdx.x / quads, r = threadIdx.x % quads * 4;
+    const int entry = m < g.M ? __ldcg(g.list.entry + m) : -1;
+    const float scale = entry >= 0 && g.scale ? g.scale[g.row_adapter[m]] : 1.0f;
     if (threadIdx.x < 32) scan_lists(g, blocks, threadIdx.x, before);
     __syncthreads();
-    const Cut cut(before[blocks], (g.K + 63) / 64, g.sms, g.parts_u);
-    const int quads = g.rank / 4;
     bool fits = true;
-    for (int i = threadIdx.x; i < 32 * quads; i += 256) {
-        const int m = blockIdx.x * 32 + i / quads, r = i % quads * 4;
-        const int entry = m < g.M ? __ldcg(g.list.entry + m) : -1;
-        if (entry < 0) continue;
+    if (entry >= 0) {
+        const Cut cut(before[blocks], (g.K + 63) / 64, g.sms, g.parts_u);
         const int parts = cut.num_parts(before[m >> 8] + entry);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int p = 0; p < parts; ++p) {
-            const float4 w = __ldcg(reinterpret_cast<const float4 *>(g.u_parts + (static_cast<int64_t>(p) * g.M + m) * g.rank + r));
-            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        const float *const src = g.u_parts + static_cast<int64_t>(m) * g.rank + r;
+        const int64_t pitch = static_cast<int64_t>(g.M) * g.rank;
+        float f[4] = {};
+        for (int p0 = 0; p0 < parts; p0 += 8) {
+            float4 w[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) w[p] = p0 + p < parts ? __ldcg(reinterpret_cast<const float4 *>(src + (p0 + p) * pitch)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int p = 0; p < 8; ++p) f[0] += w[p].x, f[1] += w[p].y, f[2] += w[p].z, f[3] += w[p].w;
         }
-        const float scale = g.scale ? g.scale[g.row_adapter[m]] : 1.0f;
-        const float f[4] = {scale * v.x, scale * v.y, scale * v.z, scale * v.w};
-        *reinterpret_cast<float4 *>(g.u + static_cast<int64_t>(m) * g.rank + r) = make_float4(f[0], f[1], f[2], f[3]);
         uint16_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            f[j] *= scale;
             T::split(f[j], hi[j], lo[j]);
             fits = fits && fabsf(f[j]) <= T::kMax;
         }
+        *reinterpret_cast<float4 *>(g.u + static_cast<int64_t>(m) * g.rank + r) = make_float4(f[0], f[1], f[2], f[3]);
         *reinterpret_cast<uint2 *>(g.u16 + static_cast<int64_t>(m) * g.rank + r) = make_uint2(hi[0] | static_cast<uint32_t>(hi[1]) << 16, hi[2] | static_cast<uint32_t>(hi[3]) << 16);
         *reinterpret_cast<uint2 *>(g.u16 + (static_cast<int64_t>(g.M) + m) * g.rank + r) = make_uint2(lo[0] | static_cast<uint32_t>(lo[1]) << 16, lo[2] | static_cast<uint32_t>(lo[3]) << 16);
     }
@@ -868,7 +888,7 @@ cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
     } else {
         e = launch(lora_list_kernel, g, (g.M + 255) / 256, 256, 0, 1, stream);
         if (e == cudaSuccess) e = launch(lora_shrink_kernel, g, g.sms, kShrinkThreads, kShrinkSmem, 1, stream);
-        if (e == cudaSuccess) e = launch(lora_join_kernel<T>, g, (g.M + 31) / 32, 256, 0, 1, stream);
+        if (e == cudaSuccess) e = launch(lora_join_kernel<T>, g, (g.M + 31) / 32, 32 * (g.rank / 4), 0, 1, stream);
     }
     if (e != cudaSuccess) return e;
     if (g.M <= kOneCtaRows) return launch(lora_product_kernel<T, 1, false>, g, g.sms, kLoraThreads, smem, 1, stream);
