@@ -35,12 +35,12 @@ constexpr int kLoraStages = 12;
 constexpr int kDeltaWarps = 8;
 constexpr int kLoraThreads = (2 + 4 + kDeltaWarps + 1) * 32;
 constexpr int kChunkRows = 16;                             // rows of D in a piece of the adapters' product
-constexpr int kMaxChunks = 8;                              // most pieces on their way to the draining warps
+constexpr int kChunks = 8;                                 // pieces on their way to the draining warps
 constexpr int kAhead = 4;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
 constexpr int kOneCtaRows = 64;                            // most rows of the one-CTA form
 constexpr int kFewRows = 256;                              // most rows that one tile takes
-constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kMaxChunks + 2 * kAhead;
+constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kChunks + 2 * kAhead;
 constexpr int kNoRow = -2;                                 // in the place of an adapter: behind the last row
 constexpr int kMaxLoraParts = 16;
 constexpr int kMaxCtas = 256;
@@ -72,7 +72,7 @@ struct alignas(64) LoraArgs {
     int wide_b;                    // rows of lora_b are whole 32-byte sectors
     int parts, sms;
     int rows;                      // of a tile: columns of an accumulator
-    int u_pitch, chunks;           // floats from row to row of u in shared memory; pieces in flight
+    int u_pitch;                   // floats from row to row of u in shared memory
     int a_bytes, stages, off_delta, off_u, off_ids, off_bars, off_misc;
     int tmem_cols;
     uint32_t idesc;
@@ -517,10 +517,16 @@ __device__ __forceinline__ bool next_run(const Groups &v, int &at, int &from, in
     return true;
 }
 
-// Whether piece c of a tile is one that the delta warps compute for this part of it: with few rows all are, the parts of a tile share them.
+// With few rows the parts of a tile share its pieces; a single piece they share by its rows, four at a time.
+__device__ __forceinline__ bool own_rows(const LoraArgs &g, const LoraSegment &s, int row) {
+    return (g.M <= kChunkRows ? row >> 2 : row / kChunkRows) % s.parts == s.part;
+}
+
+// Whether the delta warps compute something of piece c for this part of the tile.
 template <bool WAVES>
-__device__ __forceinline__ bool has_piece(const LoraSegment &s, const Groups &v, int c) {
-    return WAVES ? (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u : c % s.parts == s.part;
+__device__ __forceinline__ bool has_piece(const LoraArgs &g, const LoraSegment &s, const Groups &v, int c) {
+    if (WAVES) return (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u;
+    return g.M <= kChunkRows ? s.part < 4 : own_rows(g, s, c * kChunkRows);
 }
 
 // The pieces of one CTA in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
@@ -540,7 +546,7 @@ struct PieceWalker {
                 rows = min(g.rows, g.M - s.m0);
                 c = 0;
             }
-            if (has_piece<WAVES>(s, v, c)) return true;
+            if (has_piece<WAVES>(g, s, v, c)) return true;
         }
     }
 };
@@ -555,8 +561,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     float *const u_s = reinterpret_cast<float *>(sm + g.off_u);
     int *const id_s = reinterpret_cast<int *>(sm + g.off_ids);
     const uint32_t full0 = ring + g.off_bars, empty0 = full0 + 8 * kLoraStages, acc_full0 = empty0 + 8 * kLoraStages, acc_empty0 = acc_full0 + 16,
-                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kMaxChunks,
-                   u_full0 = delta_empty0 + 8 * kMaxChunks, u_empty0 = u_full0 + 8 * kAhead;
+                   delta_full0 = acc_empty0 + 16, delta_empty0 = delta_full0 + 8 * kChunks,
+                   u_full0 = delta_empty0 + 8 * kChunks, u_empty0 = u_full0 + 8 * kAhead;
     volatile int *const misc = reinterpret_cast<volatile int *>(sm + g.off_misc);   // abort flag, tensor-memory base, two tiles whose parts this CTA adds
     const WaitCtx wait = {g.status, misc, g.budget};
     const int tid = threadIdx.x, lane = tid & 31;
@@ -565,8 +571,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
 
     if (tid < kLoraBars) {
         // accumulators: full, empty (the draining warps of the pair); pieces: full (the delta warps), empty (the draining warps); u: full, empty
-        const int j = tid - 2 * kLoraStages, i = j - 4 - 2 * kMaxChunks;
-        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kMaxChunks ? kDeltaWarps : i < 0 ? 4 : i < kAhead ? 1 : kDeltaWarps);
+        const int j = tid - 2 * kLoraStages, i = j - 4 - 2 * kChunks;
+        mbar_init(full0 + 8 * tid, j < 2 ? 1 : j < 4 ? 4 * CG : j < 4 + kChunks ? kDeltaWarps : i < 0 ? 4 : i < kAhead ? 1 : kDeltaWarps);
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0, misc[2] = misc[3] = -1;
@@ -710,7 +716,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             for (int c = 0; c * kChunkRows < rows; ++c) {
                 uint32_t v[16];
                 tmem_ld_32x16(tmem + acc * g.rows + c * kChunkRows + (static_cast<uint32_t>(quarter * 32) << 16), v);
-                const bool add = has_piece<WAVES>(s, v_groups, c);
+                const bool add = has_piece<WAVES>(g, s, v_groups, c);
                 if (add) ok = wait_warp(delta_full0 + 8 * slot, slot_ph, wait, 2400 + slot);
                 tmem_ld_wait();
                 if (!ok) break;
@@ -720,7 +726,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                         v[j] = __float_as_uint(__uint_as_float(v[j]) + delta[(slot * kChunkRows + j) * 128 + r]);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(delta_empty0 + 8 * slot);
-                    if (++slot == g.chunks) slot = 0, slot_ph ^= 1u;
+                    if (++slot == kChunks) slot = 0, slot_ph ^= 1u;
                 }
                 if (mine) {
                     const int64_t row = s.m0 + c * kChunkRows;
@@ -783,7 +789,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 mbar_arrive(delta_full0 + 8 * slot);
             }
             if (++from == kAhead) from = 0, from_ph ^= 1u;
-            if (++slot == g.chunks) slot = 0, slot_ph ^= 1u;
+            if (++slot == kChunks) slot = 0, slot_ph ^= 1u;
         }
     } else {
         // -------------------------------------------------------------- u and the rows' adapters for the warps above
@@ -794,7 +800,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         while (ok && at.next(g, lane)) {
             const int m = at.s.m0 + at.c * kChunkRows + lane;
             const bool there = lane < kChunkRows && m < g.M;
-            const int id = lane < kChunkRows ? row_adapter(g, m) : kNoRow;
+            int id = lane < kChunkRows ? row_adapter(g, m) : kNoRow;
+            if (!WAVES && !own_rows(g, at.s, at.c * kChunkRows + lane)) id = -1;
             if (id >= 0) {
                 // what the piece will read of the adapter: 128 of its columns, which lie behind one another
                 const int col = (at.s.tile * CG + static_cast<int>(rank)) * 128;
@@ -1016,12 +1023,11 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
     g.a_bytes = box_a * 128;
     g.u_pitch = rank + 4;   // rows of u start 16 bytes further each, modulo the banks
-    g.chunks = M > 128 || rank > 64 ? 4 : kMaxChunks;
-    const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, rest = g.chunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
-    g.stages = ((M > kFewRows ? kSmemLimit : 196 * 1024) - 1024 - rest) / (128 * 128 + g.a_bytes);
+        const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, rest = kChunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
+    g.stages = (kSmemLimit - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
-    g.off_u = g.off_delta + g.chunks * kChunkBytes;
+    g.off_u = g.off_delta + kChunks * kChunkBytes;
     g.off_ids = g.off_u + u_bytes;
     g.off_bars = g.off_ids + kAhead * kChunkRows * 4;
     g.off_misc = g.off_bars + kLoraBars * 8;
