@@ -391,14 +391,15 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
 // K blocks [kb0, kb1) of the tile at row m0 and 128-column (pair: 256-column) tile `tile`, as part `part` of `parts`.
 struct LoraSegment {
     int tile, m0, kb0, kb1, part, parts;
+    int own0, own1, row0, row1;    // few rows: the pieces that this part adds; where there is one piece, its rows / 4
 };
 
 template <int CG, bool WAVES>
 struct LoraWalker {
-    int q, end, step, tiles_n, row_blocks, kblocks, rows, group;   // group: a CTA or a pair
+    int q, end, step, tiles_n, row_blocks, kblocks, rows, m, group;   // group: a CTA or a pair
     Cut cut;
     __device__ __forceinline__ LoraWalker(const LoraArgs &g)
-        : tiles_n((g.N + 128 * CG - 1) / (128 * CG)), row_blocks((g.M + g.rows - 1) / g.rows), kblocks((g.K + 63) / 64), rows(g.rows),
+        : tiles_n((g.N + 128 * CG - 1) / (128 * CG)), row_blocks((g.M + g.rows - 1) / g.rows), kblocks((g.K + 63) / 64), rows(g.rows), m(g.M),
           group(blockIdx.x / CG), cut(WAVES ? 0 : tiles_n, kblocks, gridDim.x / CG, g.parts) {
         if (WAVES) {
             q = group;
@@ -419,6 +420,16 @@ struct LoraWalker {
             s.part = group - cut.first_cta(s.tile);
             s.parts = cut.num_parts(s.tile);
             q += s.kb1 - s.kb0;
+            const int pieces = (m + kChunkRows - 1) / kChunkRows;
+            s.own0 = pieces * s.kb0 / kblocks;
+            s.own1 = pieces * s.kb1 / kblocks;
+            if (pieces == 1) {
+                const int fours = (m + 3) / 4;
+                s.row0 = fours * s.kb0 / kblocks;
+                s.row1 = fours * s.kb1 / kblocks;
+                s.own0 = 0;
+                s.own1 = s.row1 > s.row0;
+            }
         } else {
             const int in_group = kGroupRows * tiles_n, first = q / in_group * kGroupRows;
             const int height = min(row_blocks - first, kGroupRows), i = q % in_group;
@@ -517,16 +528,11 @@ __device__ __forceinline__ bool next_run(const Groups &v, int &at, int &from, in
     return true;
 }
 
-// With few rows the parts of a tile share its pieces; a single piece they share by its rows, four at a time.
-__device__ __forceinline__ bool own_rows(const LoraArgs &g, const LoraSegment &s, int row) {
-    return (g.M <= kChunkRows ? row >> 2 : row / kChunkRows) % s.parts == s.part;
-}
-
-// Whether the delta warps compute something of piece c for this part of the tile.
+// Whether the delta warps compute something of piece c for this part of the tile. With few rows the parts of a tile share its pieces, and a
+// single piece by its rows, four at a time: each as many as its share of the K blocks, so that every CTA has the same to do.
 template <bool WAVES>
-__device__ __forceinline__ bool has_piece(const LoraArgs &g, const LoraSegment &s, const Groups &v, int c) {
-    if (WAVES) return (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u;
-    return g.M <= kChunkRows ? s.part < 4 : own_rows(g, s, c * kChunkRows);
+__device__ __forceinline__ bool has_piece(const LoraSegment &s, const Groups &v, int c) {
+    return WAVES ? (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u : c >= s.own0 && c < s.own1;
 }
 
 // The pieces of one CTA in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
@@ -546,7 +552,7 @@ struct PieceWalker {
                 rows = min(g.rows, g.M - s.m0);
                 c = 0;
             }
-            if (has_piece<WAVES>(g, s, v, c)) return true;
+            if (has_piece<WAVES>(s, v, c)) return true;
         }
     }
 };
@@ -716,7 +722,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             for (int c = 0; c * kChunkRows < rows; ++c) {
                 uint32_t v[16];
                 tmem_ld_32x16(tmem + acc * g.rows + c * kChunkRows + (static_cast<uint32_t>(quarter * 32) << 16), v);
-                const bool add = has_piece<WAVES>(g, s, v_groups, c);
+                const bool add = has_piece<WAVES>(s, v_groups, c);
                 if (add) ok = wait_warp(delta_full0 + 8 * slot, slot_ph, wait, 2400 + slot);
                 tmem_ld_wait();
                 if (!ok) break;
@@ -801,7 +807,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             const int m = at.s.m0 + at.c * kChunkRows + lane;
             const bool there = lane < kChunkRows && m < g.M;
             int id = lane < kChunkRows ? row_adapter(g, m) : kNoRow;
-            if (!WAVES && !own_rows(g, at.s, at.c * kChunkRows + lane)) id = -1;
+            if (!WAVES && g.M <= kChunkRows && (lane < 4 * at.s.row0 || lane >= 4 * at.s.row1)) id = -1;
             if (id >= 0) {
                 // what the piece will read of the adapter: 128 of its columns, which lie behind one another
                 const int col = (at.s.tile * CG + static_cast<int>(rank)) * 128;
