@@ -258,58 +258,41 @@ def gemm(A, Bt, Cm=None, D=None, alpha=1.0, beta=0.0, params: Params | None = No
 
 
 _CODES = {}   # torch dtype -> B200_F16 / B200_BF16, filled on first use
+_NEEDS = {}   # sizes of a call -> bytes of its workspace
 
 
-def _code(where: str, t) -> int:
-    if not _CODES:
-        import torch
-        _CODES.update({torch.float16: F16, torch.bfloat16: BF16})
-    code = _CODES.get(t.dtype)
-    if code is None or not t.is_cuda:
-        raise ValueError(f"{where}: the operands must be fp16 or bf16 CUDA tensors, not {t.dtype} on {t.device}")
-    return code
-
-
-def _check(where: str, name: str, t, dtype, shape, device) -> None:
-    if not (t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous()):
-        raise ValueError(f"{where}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
-                         f"not {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
-
-
-def _on_stream(fn, args, device, stream):
-    """fn(*args, handle) with the tensors' device and the stream of the call current, so that what fn allocates (outputs, the
-    workspace) belongs to that stream's memory. Both usually are current already."""
+def _torch():
     import torch
+    if not _CODES:
+        _CODES.update({torch.float16: F16, torch.bfloat16: BF16})
+    return torch
+
+
+def _refuse(where: str, first, named) -> None:
+    """Says which tensor of a call does not fit. named: (name, tensor, dtype, shape); a tensor of None is not given."""
+    if first.dtype not in _CODES or not first.is_cuda:
+        raise ValueError(f"{where}: the operands must be fp16 or bf16 CUDA tensors, not {first.dtype} on {first.device}")
+    for name, t, dtype, shape in named:
+        if t is not None and not (t.shape == shape and t.dtype == dtype and t.device == first.device and t.is_contiguous()):
+            raise ValueError(f"{where}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {first.device}, "
+                             f"not {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
+    raise ValueError(f"{where}: the tensors do not fit together")
+
+
+def _other_stream(torch, device, stream):
+    """The context of a call on another device or stream than the current ones: what it allocates (outputs, the workspace) belongs to
+    that stream's memory. None where both are current, the usual case; and the stream's handle."""
     raw = torch._C._cuda_getCurrentRawStream(device.index)
     handle = raw if stream is None else int(stream)
     if handle == raw and device.index == torch.cuda.current_device():
-        return fn(*args, handle)
+        return None, handle
     on = torch.cuda.current_stream(device) if handle == raw else torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
-    with torch.cuda.stream(on):
-        return fn(*args, handle)
+    return torch.cuda.stream(on), handle
 
 
 def gemm_lora_workspace_bytes(M, N, K, num_adapters, rank) -> int:
     """b200_gemm_lora_workspace_bytes; -1 for sizes that the call refuses."""
     return lib().b200_gemm_lora_workspace_bytes(M, N, K, num_adapters, rank)
-
-
-def _gemm_lora(code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, sizes, stream):
-    import torch
-    M, N, K, S, R = sizes
-    L = lib()
-    if workspace is None:
-        need = L.b200_gemm_lora_workspace_bytes(M, N, K, S, R)
-        if need > 0:
-            workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=A.device)   # the quickest of torch's allocations
-    if D is None:
-        D = torch.empty_strided((M, N), (N, 1), dtype=A.dtype, device=A.device)
-    st = L.b200_gemm_lora(code, A.data_ptr(), Bt.data_ptr(), D.data_ptr(), M, N, K, lora_a.data_ptr(), lora_b.data_ptr(),
-                          lora_scale.data_ptr() if lora_scale is not None else None, row_adapter.data_ptr(), S, R,
-                          workspace.data_ptr() if workspace is not None else None, workspace.nbytes if workspace is not None else 0, stream)
-    if st != OK:
-        raise B200Error(st, "b200_gemm_lora")
-    return D
 
 
 def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, workspace=None, stream=None):
@@ -321,46 +304,49 @@ def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, works
     D and the workspace are allocated, on the stream of the call, when not given. stream: a cudaStream_t as an int (None =
     torch's current one); the operands must be ready there. Raises ValueError for tensors that do not fit together and
     B200Error for what the library refuses."""
-    import torch
-    code = _code("gemm_lora", A)
+    torch = _torch()
     if A.dim() != 2 or Bt.dim() != 2 or lora_a.dim() != 3:
         raise ValueError("gemm_lora: A and Bt must have 2 dimensions and lora_a 3")
-    (M, K), N, (S, R, _), dev, t, i32 = A.shape, Bt.shape[0], lora_a.shape, A.device, A.dtype, torch.int32
-    _check("gemm_lora", "A", A, t, (M, K), dev)
-    _check("gemm_lora", "Bt", Bt, t, (N, K), dev)
-    _check("gemm_lora", "lora_a", lora_a, t, (S, R, K), dev)
-    _check("gemm_lora", "lora_b", lora_b, t, (S, N, R), dev)
-    _check("gemm_lora", "row_adapter", row_adapter, i32, (M,), dev)
-    if lora_scale is not None:
-        _check("gemm_lora", "lora_scale", lora_scale, torch.float32, (S,), dev)
-    if D is not None:
-        _check("gemm_lora", "D", D, t, (M, N), dev)
-    return _on_stream(_gemm_lora, (code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, (M, N, K, S, R)), dev, stream)
+    (M, K), N, (S, R, _), dev, t = A.shape, Bt.shape[0], lora_a.shape, A.device, A.dtype
+    code = _CODES.get(t)
+    if not (code is not None and A.is_cuda and A.is_contiguous()
+            and Bt.shape == (N, K) and Bt.dtype is t and Bt.device == dev and Bt.is_contiguous()
+            and lora_a.shape == (S, R, K) and lora_a.dtype is t and lora_a.device == dev and lora_a.is_contiguous()
+            and lora_b.shape == (S, N, R) and lora_b.dtype is t and lora_b.device == dev and lora_b.is_contiguous()
+            and row_adapter.shape == (M,) and row_adapter.dtype is torch.int32 and row_adapter.device == dev and row_adapter.is_contiguous()
+            and (lora_scale is None or lora_scale.shape == (S,) and lora_scale.dtype is torch.float32 and lora_scale.device == dev and lora_scale.is_contiguous())
+            and (D is None or D.shape == (M, N) and D.dtype is t and D.device == dev and D.is_contiguous())
+            and (workspace is None or workspace.device == dev and workspace.is_contiguous())):
+        _refuse("gemm_lora", A, (("A", A, t, (M, K)), ("Bt", Bt, t, (N, K)), ("lora_a", lora_a, t, (S, R, K)), ("lora_b", lora_b, t, (S, N, R)),
+                                 ("row_adapter", row_adapter, torch.int32, (M,)), ("lora_scale", lora_scale, torch.float32, (S,)), ("D", D, t, (M, N))))
+    on, handle = _other_stream(torch, dev, stream)
+    if on is not None:
+        with on:
+            return _gemm_lora(torch, code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, M, N, K, S, R, handle)
+    return _gemm_lora(torch, code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, M, N, K, S, R, handle)
+
+
+def _gemm_lora(torch, code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, M, N, K, S, R, stream):
+    L = _lib or lib()
+    if workspace is None:
+        need = _NEEDS.get((M, N, K, R))
+        if need is None:
+            need = max(L.b200_gemm_lora_workspace_bytes(M, N, K, S, R), 0)
+            if need and len(_NEEDS) < 4096:
+                _NEEDS[M, N, K, R] = need
+        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=A.device)   # the quickest of torch's allocations
+    if D is None:
+        D = torch.empty_strided((M, N), (N, 1), dtype=A.dtype, device=A.device)
+    st = L.b200_gemm_lora(code, A.data_ptr(), Bt.data_ptr(), D.data_ptr(), M, N, K, lora_a.data_ptr(), lora_b.data_ptr(),
+                          None if lora_scale is None else lora_scale.data_ptr(), row_adapter.data_ptr(), S, R, workspace.data_ptr(), workspace.nbytes, stream)
+    if st != OK:
+        raise B200Error(st, "b200_gemm_lora")
+    return D
 
 
 def moe_workspace_bytes(tokens, hidden, inner, experts, top_k) -> int:
     """b200_moe_workspace_bytes; -1 for sizes that the call refuses."""
     return lib().b200_moe_workspace_bytes(tokens, hidden, inner, experts, top_k)
-
-
-def _moe(code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, sizes, stream):
-    import torch
-    T, H, I, E, k = sizes
-    L = lib()
-    if workspace is None:
-        need = max(L.b200_moe_workspace_bytes(T, H, I, E, k), 0)
-        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=X.device)   # the quickest of torch's allocations
-    if Y is None:
-        Y = torch.empty_like(X)
-    if ids is None:
-        ids = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.int32, device=X.device)
-    if weights is None:
-        weights = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.float32, device=X.device)
-    st = L.b200_moe(code, X.data_ptr(), logits.data_ptr(), W13.data_ptr(), W2.data_ptr(), Y.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, H, I, E,
-                    k, 1 if normalise else 0, workspace.data_ptr(), workspace.nbytes, stream)
-    if st != OK:
-        raise B200Error(st, "b200_moe")
-    return Y, ids, weights
 
 
 def moe(X, logits, W13, W2, top_k, normalise=True, Y=None, ids=None, weights=None, workspace=None, stream=None):
@@ -371,22 +357,49 @@ def moe(X, logits, W13, W2, top_k, normalise=True, Y=None, ids=None, weights=Non
     product; ids (tokens, top_k) int32 and weights (tokens, top_k) fp32 are the router's choice, in descending order of the
     logits. Outputs and the workspace are allocated, on the stream of the call, when not given; stream as in gemm_lora.
     Raises ValueError for tensors that do not fit together and B200Error for what the library refuses."""
-    import torch
-    code = _code("moe", X)
+    torch = _torch()
     if X.dim() != 2 or W2.dim() != 3:
         raise ValueError("moe: X must have 2 dimensions and W2 3")
-    (T, H), (E, _, I), dev, t, f32 = X.shape, W2.shape, X.device, X.dtype, torch.float32
-    _check("moe", "X", X, t, (T, H), dev)
-    _check("moe", "logits", logits, f32, (T, E), dev)
-    _check("moe", "W13", W13, t, (E, 2 * I, H), dev)
-    _check("moe", "W2", W2, t, (E, H, I), dev)
-    if Y is not None:
-        _check("moe", "Y", Y, t, (T, H), dev)
-    if ids is not None:
-        _check("moe", "ids", ids, torch.int32, (T, top_k), dev)
-    if weights is not None:
-        _check("moe", "weights", weights, f32, (T, top_k), dev)
-    return _on_stream(_moe, (code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, (T, H, I, E, top_k)), dev, stream)
+    (T, H), (E, _, I), dev, t = X.shape, W2.shape, X.device, X.dtype
+    code = _CODES.get(t)
+    if not (code is not None and X.is_cuda and X.is_contiguous()
+            and logits.shape == (T, E) and logits.dtype is torch.float32 and logits.device == dev and logits.is_contiguous()
+            and W13.shape == (E, 2 * I, H) and W13.dtype is t and W13.device == dev and W13.is_contiguous()
+            and W2.shape == (E, H, I) and W2.dtype is t and W2.device == dev and W2.is_contiguous()
+            and (Y is None or Y.shape == (T, H) and Y.dtype is t and Y.device == dev and Y.is_contiguous())
+            and (ids is None or ids.shape == (T, top_k) and ids.dtype is torch.int32 and ids.device == dev and ids.is_contiguous())
+            and (weights is None or weights.shape == (T, top_k) and weights.dtype is torch.float32 and weights.device == dev and weights.is_contiguous())
+            and (workspace is None or workspace.device == dev and workspace.is_contiguous())):
+        _refuse("moe", X, (("X", X, t, (T, H)), ("logits", logits, torch.float32, (T, E)), ("W13", W13, t, (E, 2 * I, H)), ("W2", W2, t, (E, H, I)),
+                           ("Y", Y, t, (T, H)), ("ids", ids, torch.int32, (T, top_k)), ("weights", weights, torch.float32, (T, top_k))))
+    on, handle = _other_stream(torch, dev, stream)
+    if on is not None:
+        with on:
+            return _moe(torch, code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, T, H, I, E, top_k, handle)
+    return _moe(torch, code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, T, H, I, E, top_k, handle)
+
+
+def _moe(torch, code, X, logits, W13, W2, normalise, Y, ids, weights, workspace, T, H, I, E, k, stream):
+    L = _lib or lib()
+    dev = X.device
+    if workspace is None:
+        need = _NEEDS.get((T, H, I, E, k))
+        if need is None:
+            need = max(L.b200_moe_workspace_bytes(T, H, I, E, k), 0)
+            if need and len(_NEEDS) < 4096:
+                _NEEDS[T, H, I, E, k] = need
+        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)   # the quickest of torch's allocations
+    if Y is None:
+        Y = torch.empty_like(X)
+    if ids is None:
+        ids = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.int32, device=dev)
+    if weights is None:
+        weights = torch.empty_strided((T, max(k, 0)), (max(k, 0), 1), dtype=torch.float32, device=dev)
+    st = L.b200_moe(code, X.data_ptr(), logits.data_ptr(), W13.data_ptr(), W2.data_ptr(), Y.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, H, I, E, k,
+                    1 if normalise else 0, workspace.data_ptr(), workspace.nbytes, stream)
+    if st != OK:
+        raise B200Error(st, "b200_moe")
+    return Y, ids, weights
 
 
 def device_status(stream=None):
