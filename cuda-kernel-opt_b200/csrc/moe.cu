@@ -52,6 +52,7 @@ struct Lists {
     int *count;
     int *base;
     int *token;      // per slot (sorted by expert, then token): its token
+    int *owner;      // per slot: the position of its expert in the list of chosen ones
     int *slot;       // per (token, choice): its slot, -1 without one
     int *active;     // per (token, choice): the position of its expert in the list of chosen ones
     float *weight;   // per (token, choice)
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__
         if (e < 0) continue;
         const int slot = first[e] + rank_of(mask, words, e, t);
         g.list.token[slot] = t;
+        g.list.owner[slot] = place[e];
         g.list.slot[at] = slot;
         g.list.active[at] = place[e];
     }
@@ -271,6 +273,11 @@ struct Walker {
         return true;
     }
 };
+
+// 128-row atoms of the weights per tile. With more than a few tokens two share the activations of a K block, which halves what those
+// cost between L2 and SM (256 tokens, 128 experts of 2048 x 768: 0.44 GB of activations beside 0.41 GB of W2), as long as
+// two accumulators of both fit the tensor memory.
+__device__ __forceinline__ int tile_atoms(const MoeArgs &g, int most) { return 4 * ((most + 15) / 16 * 16) <= g.tmem_cols ? 2 : 1; }
 
 enum Product {
     UP,        // gate and up rows times the tokens of X, gathered by the loader warps
@@ -463,11 +470,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     const int chosen = __shfl_sync(0xffffffffu, misc[2], 0), most = __shfl_sync(0xffffffffu, misc[3], 0);
     const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[1]), 0);
 
-    const int tiles_up = (g.inner + 63) / 64, kb_up = (g.hidden + 63) / 64;
-    const int tiles = !kUp ? (g.hidden + 127) / 128 : tiles_up;
-    const Cut cut(chosen * tiles, !kUp ? tiles_up : kb_up, g.sms, !kUp ? g.parts_down : g.parts_up);
-    const uint32_t rows_bytes = static_cast<uint32_t>((most + 15) / 16 * 16 * 128);   // the activations of a K block (16-bit values)
-    const uint32_t stage_bytes = kWeightBytes + rows_bytes * (!kUp ? 2 : 1);
+    const int atoms = kFew ? 1 : tile_atoms(g, most);
+    const int blocks_up = (g.inner + 63) / 64, kb_up = (g.hidden + 63) / 64, tiles_up = (blocks_up + atoms - 1) / atoms;   // blocks: of one atom
+    const int blocks = kUp ? blocks_up : (g.hidden + 127) / 128, tiles = (blocks + atoms - 1) / atoms;
+    const Cut cut(chosen * tiles, kUp ? kb_up : blocks_up, g.sms, kUp ? g.parts_up : g.parts_down);
+    const uint32_t columns = static_cast<uint32_t>((most + 15) / 16 * 16), acc_cols = kFew ? static_cast<uint32_t>(g.slot_cols) : atoms * columns;
+    const uint32_t rows_bytes = columns * 128;             // the activations of a K block (16-bit values)
+    const uint32_t rows_at = kWeightBytes * atoms, stage_bytes = rows_at + rows_bytes * (kUp ? 1 : 2);
     const int stages = min(kMoeStages, static_cast<int>(g.ring_bytes / stage_bytes));
     Walker<P == DOWN_FEW> walk(cut, tiles, chosen, blockIdx.x);
     Segment s;
@@ -485,11 +494,11 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         if (P == DOWN) {
             // the weights of the first stages do not depend on the kernels before: on their way before the wait
             while (filled < stages && ahead.next(f)) {
-                const int row = expert_s[f.ai] * g.hidden + f.tile * 128;
+                const int row = expert_s[f.ai] * g.hidden + f.tile * atoms * 128, na = min(atoms, blocks - f.tile * atoms);
                 for (fkb = f.kb0; fkb < f.kb1 && filled < stages; ++fkb, ++filled, ++fst)
                     if (issuer) {
-                        mbar_arrive_expect_tx(full0 + 8 * fst, kWeightBytes + (count_s[f.ai] + 15) / 16 * 2 * kBoxBytes);
-                        tma_load_2d_hint(ring + fst * stage_bytes, &g.map, full0 + 8 * fst, fkb * 64, row, once);
+                        mbar_arrive_expect_tx(full0 + 8 * fst, kWeightBytes * na + (count_s[f.ai] + 15) / 16 * 2 * kBoxBytes);
+                        for (int a = 0; a < na; ++a) tma_load_2d_hint(ring + fst * stage_bytes + a * kWeightBytes, &g.map, full0 + 8 * fst, fkb * 64, row + a * 128, once);
                     }
             }
             griddep_wait();
@@ -497,7 +506,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         while (ok && walk.next(s)) {
             const int e = expert_s[s.ai];
             const int boxes = (count_s[s.ai] + 15) / 16;
-            const int row = !kUp ? e * g.hidden + s.tile * 128 : e * 2 * g.inner + s.tile * 64;
+            const int row = kUp ? e * 2 * g.inner + s.tile * atoms * 64 : e * g.hidden + s.tile * atoms * 128;
+            const int na = min(atoms, blocks - s.tile * atoms);
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
                 if (P == DOWN && filled > 0) {
                     --filled;                              // its weights are on their way
@@ -506,13 +516,16 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                     if (!ok) break;
                     if (issuer) {
                         const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
-                        mbar_arrive_expect_tx(bar, kWeightBytes + (P == DOWN ? boxes * 2 * kBoxBytes : 0));
-                        tma_load_2d_hint(dst, &g.map, bar, kb * 64, row, once);
-                        if (kUp) tma_load_2d_hint(dst + kWeightBytes / 2, &g.map, bar, kb * 64, row + g.inner, once);
+                        mbar_arrive_expect_tx(bar, kWeightBytes * na + (P == DOWN ? boxes * 2 * kBoxBytes : 0));
+                        for (int a = 0; a < na; ++a) {
+                            const uint32_t to = dst + a * kWeightBytes;
+                            tma_load_2d_hint(to, &g.map, bar, kb * 64, row + a * (kUp ? 64 : 128), once);
+                            if (kUp) tma_load_2d_hint(to + kWeightBytes / 2, &g.map, bar, kb * 64, row + a * 64 + g.inner, once);
+                        }
                     }
                 }
                 if (P == DOWN && issuer) {
-                    const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes + kWeightBytes;
+                    const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes + rows_at;
                     for (int b = 0; b < boxes; ++b) {
                         tma_load_2d(dst + b * kBoxBytes, &g.map_h, bar, kb * 64, base_s[s.ai] + 16 * b);
                         tma_load_2d(dst + rows_bytes + b * kBoxBytes, &g.map_h, bar, kb * 64, g.slots + base_s[s.ai] + 16 * b);
@@ -530,19 +543,23 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
             ok = wait_warp(acc_empty0 + 8 * acc, ((n >> 1) & 1) ^ 1u, wait, 1100 + acc);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t d = tmem + acc * g.slot_cols;
+            const uint32_t d = tmem + acc * acc_cols;
+            const int na = min(atoms, blocks - s.tile * atoms);
             const uint32_t idesc = g.idesc | static_cast<uint32_t>((count_s[s.ai] + 15) / 16 * 2) << 17;
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
                 ok = wait_warp(full0 + 8 * st, ph, wait, 1200 + st);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t at = ring + st * stage_bytes;
-                const uint64_t a = umma_desc_sw128(at), b = umma_desc_sw128(at + kWeightBytes), lo = umma_desc_sw128(at + kWeightBytes + rows_bytes);
+                const uint64_t w = umma_desc_sw128(at), b = umma_desc_sw128(at + rows_at), lo = umma_desc_sw128(at + rows_at + rows_bytes);
                 if (issuer) {
+                    for (int a = 0; a < na; ++a) {
+                        const uint64_t wa = w + a * (kWeightBytes >> 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        umma_f16<1>(d, a + 2 * i, b + 2 * i, idesc, kb > s.kb0 || i > 0);
-                        if (!kUp) umma_f16<1>(d, a + 2 * i, lo + 2 * i, idesc, 1);
+                        for (int i = 0; i < 4; ++i) {
+                            umma_f16<1>(d + a * columns, wa + 2 * i, b + 2 * i, idesc, kb > s.kb0 || i > 0);
+                            if (!kUp) umma_f16<1>(d + a * columns, wa + 2 * i, lo + 2 * i, idesc, 1);
+                        }
                     }
                     umma_commit<1>(empty0 + 8 * st);
                 }
@@ -560,32 +577,36 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         for (int n = 0; ok && walk.next(s); ++n) {
             const int acc = n & 1, count = count_s[s.ai];
             const int64_t slot = static_cast<int64_t>(s.part) * g.slots + base_s[s.ai];
-            float *out;
-            int pitch;
-            bool mine;
-            if (!kUp) {
-                mine = s.tile * 128 + r < g.hidden;
-                pitch = g.hidden;
-                out = g.o + slot * pitch + s.tile * 128 + r;
-            } else {
-                const int i = s.tile * 64 + (r & 63);
-                mine = i < g.inner;
-                pitch = 2 * g.inner;
-                out = g.z + slot * pitch + (r < 64 ? i : g.inner + i);
-            }
+            const int na = min(atoms, blocks - s.tile * atoms);
             ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 1300 + acc);
             if (!ok) break;
             tc_fence_after_sync();
-            for (int c = 0; c < count; c += 16) {
-                uint32_t v[16];
-                tmem_ld_32x16(tmem + acc * g.slot_cols + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
-                tmem_ld_wait();
-                if (mine) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < count) out[static_cast<int64_t>(c + j) * pitch] = __uint_as_float(v[j]);
+            for (int a = 0; a < na; ++a) {
+                const int block = s.tile * atoms + a;
+                float *out;
+                int pitch;
+                bool mine;
+                if (kUp) {
+                    const int i = block * 64 + (r & 63);
+                    mine = i < g.inner;
+                    pitch = 2 * g.inner;
+                    out = g.z + slot * pitch + (r < 64 ? i : g.inner + i);
+                } else {
+                    mine = block * 128 + r < g.hidden;
+                    pitch = g.hidden;
+                    out = g.o + slot * pitch + block * 128 + r;
                 }
-                __syncwarp();
+                for (int c = 0; c < count; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld_32x16(tmem + acc * acc_cols + a * columns + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                    tmem_ld_wait();
+                    if (mine) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c + j < count) out[static_cast<int64_t>(c + j) * pitch] = __uint_as_float(v[j]);
+                    }
+                    __syncwarp();
+                }
             }
             tc_fence_before_sync();
             __syncwarp();
@@ -627,7 +648,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                 if (turn == mine) {
                     ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1400 + st);
                     if (!ok) break;
-                    const uint32_t dst = ring + st * stage_bytes + kWeightBytes;
+                    const uint32_t dst = ring + st * stage_bytes + rows_at;
                     const int k = kb * 64 + chunk * 8;
                     if (kUp) {
                         for (int r = row0; r < count; r += row_step) {
@@ -691,21 +712,15 @@ template <typename T>
 __global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
     griddep_launch_dependents();   // DOWN reads nothing of this kernel before its own wait
     griddep_wait();
-    const int chunks = g.inner / 4, tiles = (g.inner + 63) / 64;
-    const int at = blockIdx.x * 256 + threadIdx.x, slot = at / chunks, k = (at - slot * chunks) * 4;
-    const int chosen = __ldcg(g.list.header);
-    if (slot >= g.slots || chosen == 0) return;
-    // the expert of a slot: the last one whose first slot is not behind it
-    int lo_ai = 0, hi_ai = chosen - 1;
-    while (lo_ai < hi_ai) {
-        const int mid = (lo_ai + hi_ai + 1) >> 1;
-        if (__ldcg(g.list.base + mid) <= slot) lo_ai = mid;
-        else hi_ai = mid - 1;
-    }
-    if (slot >= __ldcg(g.list.base + lo_ai) + __ldcg(g.list.count + lo_ai)) return;
+    const int slot = blockIdx.y, k = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+    const int chosen = __ldcg(g.list.header), most = __ldcg(g.list.header + 1), owner = __ldcg(g.list.owner + slot);
+    if (k >= g.inner || chosen == 0) return;
+    // slots behind the last one are nobody's: their entries are what the workspace held
+    if (slot >= __ldcg(g.list.base + chosen - 1) + __ldcg(g.list.count + chosen - 1)) return;
+    const int atoms = tile_atoms(g, most), tiles = ((g.inner + 63) / 64 + atoms - 1) / atoms;
     const Cut up(chosen * tiles, (g.hidden + 63) / 64, g.sms, g.parts_up);
     uint2 hi, lo;
-    gated_values<T>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(lo_ai * tiles + k / 64),
+    gated_values<T>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(owner * tiles + k / 64 / atoms),
                     static_cast<int64_t>(g.slots) * 2 * g.inner, hi, lo);
     *reinterpret_cast<uint2 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = hi;
     *reinterpret_cast<uint2 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = lo;
@@ -715,19 +730,20 @@ template <typename T>
 __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ MoeArgs g) {
     __shared__ int2 entry[4][B200_MOE_MAX_TOP_K * kMaxParts];
     const int t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tile = blockIdx.x * 4 + warp, tiles = (g.hidden + 127) / 128;
+    const int block = blockIdx.x * 4 + warp, blocks = (g.hidden + 127) / 128;
     griddep_wait();
     griddep_launch_dependents();
     int slot = -1, parts = 0;
     float w = 0.0f;
     if (lane < g.top_k) {
+        const int atoms = tile_atoms(g, __ldcg(g.list.header + 1)), tiles = (blocks + atoms - 1) / atoms;
         const Cut cut(__ldcg(g.list.header) * tiles, (g.inner + 63) / 64, g.sms, g.parts_down);
         const int at = t * g.top_k + lane;
         slot = __ldcg(g.list.slot + at);
         w = __ldcg(g.list.weight + at);
-        if (slot >= 0 && tile < tiles) parts = cut.num_parts(__ldcg(g.list.active + at) * tiles + tile);
+        if (slot >= 0 && block < blocks) parts = cut.num_parts(__ldcg(g.list.active + at) * tiles + block / atoms);
     }
-    combine<T>(g, entry[warp], t, tile * 128 + lane * 4, lane, slot, parts, w);
+    combine<T>(g, entry[warp], t, block * 128 + lane * 4, lane, slot, parts, w);
 }
 
 int check_moe(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
@@ -760,7 +776,7 @@ MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t expe
     l.parts_down = most_parts(top_k * ((hidden + 127) / 128), up_tiles);
     l.off_list = 0;
     l.few = slots <= kFewSlots && tokens <= kFewTokens;
-    l.off_z = l.few ? up256((hidden + 127) / 128 * 4) : up256((2 + 3 * experts + 4 * slots) * 4);
+    l.off_z = l.few ? up256((hidden + 127) / 128 * 4) : up256((2 + 3 * experts + 5 * slots) * 4);
     l.off_o = l.off_z + up256(l.parts_up * slots * 2 * inner * 4);
     l.off_h = l.off_o + up256(l.parts_down * slots * hidden * 4);
     l.bytes = l.off_h + (l.few ? 0 : up256(2 * slots * inner * 2));
@@ -797,8 +813,8 @@ cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &dow
     const int blocks = (g.tokens + 31) / 32;
     cudaError_t e = launch(moe_route_kernel, g, blocks, 1024, 0, blocks, stream);
     if (e == cudaSuccess) e = launch(moe_product_kernel<T, UP>, g, g.sms, kMoeThreads, smem, 0, stream);
-    const int64_t chunks = static_cast<int64_t>(g.slots) * (g.inner / 4);
-    if (e == cudaSuccess) e = launch(moe_gate_kernel<T>, g, static_cast<unsigned>((chunks + 255) / 256), 256, 0, 0, stream);
+    const int quads = g.inner / 4, threads = quads >= 256 ? 256 : (quads + 31) / 32 * 32;
+    if (e == cudaSuccess) e = launch(moe_gate_kernel<T>, g, dim3((quads + threads - 1) / threads, g.slots), threads, 0, 0, stream);
     g.map = down;
     if (e == cudaSuccess) e = launch(moe_product_kernel<T, DOWN>, g, g.sms, kMoeThreads, smem, 0, stream);
     if (e == cudaSuccess) e = launch(moe_combine_kernel<T>, g, dim3((g.hidden + 511) / 512, g.tokens), 128, 0, 0, stream);
@@ -865,7 +881,8 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     g.list.count = g.list.expert + experts;
     g.list.base = g.list.count + experts;
     g.list.token = g.list.base + experts;
-    g.list.slot = g.list.token + slots;
+    g.list.owner = g.list.token + slots;
+    g.list.slot = g.list.owner + slots;
     g.list.active = g.list.slot + slots;
     g.list.weight = reinterpret_cast<float *>(g.list.active + slots);
     g.z = reinterpret_cast<float *>(ws + l.off_z);
@@ -887,7 +904,8 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     // Two accumulators of up to `tokens` columns. While the tokens are few a CTA takes less than half of an SM's shared memory,
     // so that DOWN can start beside UP; more tokens need the larger ring (a K block of DOWN is up to 80 KB then).
     g.slot_cols = static_cast<int>((tokens + 15) / 16 * 16);
-    g.tmem_cols = pow2_at_least(2 * g.slot_cols);
+    g.tmem_cols = pow2_at_least((l.few ? 2 : 4) * g.slot_cols);
+    if (g.tmem_cols > kTmemColumns) g.tmem_cols = kTmemColumns;
     const int slot_lists = static_cast<int>(up256(slots * (l.few ? 10 : 2)));
     const int expert_lists = static_cast<int>(up256(experts * (12 + (l.few ? (tokens + 31) / 32 * 4 + 2 : 0))));
     const int smem = l.few ? 113 * 1024 : kSmemLimit;   // two blocks of 114 KB each are an SM's 228
