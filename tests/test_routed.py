@@ -431,6 +431,102 @@ def test_chains_without_pauses_keep_their_order(pkg, cuda):
         assert torch.equal(slow, fast) and bool(slow.isfinite().all())
 
 
+# ------------------------------------------------------------------------------------------------ far corners
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [20, 100, 400])
+def test_lora_first_product_beyond_the_range_of_fp16(pkg, cuda, m):
+    """u is held in fp32: values that fp16 has no number for (here up to some 10^6) meet small weights and give ordinary results."""
+    torch = cuda
+    x, w, a, b, scale = lora_inputs(torch, "fp16", m, 264, 512, 16, 2, m)
+    x, a, b = x * 30.0, a * 8000.0, b * 1e-4
+    ids = (torch.arange(m, device="cuda") >= m // 2).to(torch.int32)
+    u = torch.stack([x[i].double() @ a[ids[i]].double().t() for i in range(0, m, 7)])
+    assert float(u.abs().max()) > 2 * 65504
+    got = run_lora(pkg, torch, x, w, a, b, ids, scale)
+    check_close(got, *lora_want(torch, x, w, a, b, ids, scale), "fp16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [2, 150])
+def test_moe_gated_values_beyond_the_range_of_fp16(pkg, cuda, tokens):
+    """A gated value travels as a pair of 16-bit numbers: up to twice the largest fp16 in that type."""
+    torch = cuda
+    x, logits, w13, w2 = moe_inputs(torch, "fp16", tokens, 264, 72, 6, tokens)
+    w13, w2 = w13 * 50.0, w2 * 1e-3
+    x[:, 0] = 8.0
+    w13[:, 5, :] = 0
+    w13[:, 5, 0] = 40.0                      # gate of inner row 5: 320
+    w13[:, 72 + 5, :] = 0
+    w13[:, 72 + 5, 0] = 50.0                 # its other half: 400, so the gated value is 128000
+    check_moe(pkg, torch, "fp16", x, logits, w13, w2, 2, True)
+
+
+@pytest.mark.gpu
+def test_lora_more_rows_than_one_pass_and_offsets_past_32_bits(pkg, cuda):
+    """70000 rows are two passes of the library; D has more than 2^31 elements."""
+    torch = cuda
+    m, n, k, r, s = 70000, 32768, 64, 8, 5
+    x, w, a, b, scale = lora_inputs(torch, "bf16", m, n, k, r, s, 3)
+    ids = ((torch.arange(m, device="cuda") // 97) % (s + 1) - 1).to(torch.int32)
+    D = torch.empty(m, n, dtype=x.dtype, device="cuda")
+    D[-1, -8:] = float("nan")
+    assert D.numel() > 2 ** 31
+    pkg.gemm_lora(x, w, a, b, ids, scale, D=D)
+    assert pkg.device_status()[0] == pkg.OK
+    rows = torch.cat([torch.arange(0, m, 1999, device="cuda"), torch.arange(65500, 65600, device="cuda"), torch.arange(m - 40, m, device="cuda")])
+    check_close(D[rows], *lora_want(torch, x[rows], w, a, b, ids[rows], scale), "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_moe_weights_past_32_bits(pkg, cuda, tokens):
+    """W13 has more than 2^32 elements, W2 more than 2^31; the chosen experts lie at both ends."""
+    torch = cuda
+    experts, inner, hidden = 512, 1040, 4096
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w13 = torch.empty(experts, 2 * inner, hidden, dtype=torch.bfloat16, device="cuda").normal_(0, hidden ** -0.5, generator=g)
+    w2 = torch.empty(experts, hidden, inner, dtype=torch.bfloat16, device="cuda").normal_(0, inner ** -0.5, generator=g)
+    assert w13.numel() > 2 ** 32 and w2.numel() > 2 ** 31
+    x = torch.randn(tokens, hidden, generator=g, device="cuda").bfloat16()
+    logits = torch.randn(tokens, experts, generator=g, device="cuda")
+    logits[:, [0, 300, 511]] += 20.0
+    y, ids, weights = run_moe(pkg, torch, x, logits, w13, w2, 3, True)
+    assert sorted(set(ids.flatten().tolist())) == [0, 300, 511]
+    want_ids, want_weights = route_want(torch, logits, 3, True)
+    assert torch.equal(ids, want_ids)
+    used = [0, 300, 511]
+    place = torch.full((experts,), -1, dtype=torch.int32, device="cuda")
+    place[used] = torch.arange(3, dtype=torch.int32, device="cuda")
+    check_close(y, *moe_want(torch, x, w13[used], w2[used], place[want_ids.long()], want_weights), "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["lora 8", "lora 100", "lora 600", "moe 2", "moe 200"])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(pkg, cuda, op):
+    """With a budget of a nanosecond some bounded wait of the call expires: the launch ends by itself, the status record says so, and the
+    same call with the usual budget is correct. The sizes make a wait longer than the hardware suspends a warp for on its own."""
+    torch = cuda
+    name, rows = op.split()
+    if name == "lora":
+        x, w, a, b, scale = lora_inputs(torch, "bf16", int(rows), 8192, 131072, 16, 3, 5)
+        ids = lora_ids(torch, "stretches", int(rows), 3, 6)
+        call = lambda: pkg.gemm_lora(x, w, a, b, ids, scale)
+    else:
+        x, logits, w13, w2 = moe_inputs(torch, "bf16", int(rows), 16384, 16384, 2, 5)
+        call = lambda: pkg.moe(x, logits, w13, w2, 1)[0]
+    want = call()
+    assert pkg.device_status()[0] == pkg.OK
+    pkg.set_wait_budget_ns(1)
+    try:
+        call()
+        status, info = pkg.device_status()
+    finally:
+        pkg.set_wait_budget_ns(2_000_000_000)
+    assert status == pkg.DEVICE_TIMEOUT and 1000 <= info[2] < 3400, (status, info)
+    assert torch.equal(call(), want) and pkg.device_status()[0] == pkg.OK
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 
 def test_lora_refusals(pkg):
