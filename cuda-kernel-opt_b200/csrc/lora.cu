@@ -447,13 +447,50 @@ struct LoraWalker {
 
 // Rows with adapters of their own: one column n per lane, four rows at a time, fp32 on pairs of ranks. The rows' adapters are read 32
 // ranks at a time: 16 loads of 16 bytes (or 8 of a whole sector) in flight per lane.
-template <typename T>
+template <typename T, bool WAVES>
 __device__ __forceinline__ void four_rows(const LoraArgs &g, const int4 id, const float *u, int pitch, int n, float *d) {
     const int rank = g.rank, s[4] = {id.x, id.y, id.z, id.w};
     const bool wide = g.wide_b != 0;
     float2 sum[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    const int one = max(max(s[0], s[1]), max(s[2], s[3]));
+    if (one < 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j * 128] = 0.0f;
+        return;
+    }
+    if (WAVES && (s[0] < 0 || s[0] == one) && (s[1] < 0 || s[1] == one) && (s[2] < 0 || s[2] == one) && (s[3] < 0 || s[3] == one)) {
+        // one adapter among them, the usual case where requests bring several rows: all of its ranks in one go
+        const uint4 *const p = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(one) * g.N + n) * rank);
+        uint4 b[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            if (8 * i >= rank) break;
+            if (wide) ld_32(p + i, b[i], b[i + 1]);
+            else {
+                b[i] = __ldcg(p + i);
+                b[i + 1] = 8 * i + 8 < rank ? __ldcg(p + i + 1) : make_uint4(0, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (8 * i >= rank) break;
+            const float2 w0 = T::unpack(b[i].x), w1 = T::unpack(b[i].y), w2 = T::unpack(b[i].z), w3 = T::unpack(b[i].w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 f = reinterpret_cast<const float4 *>(u + j * pitch + 8 * i)[0], e = reinterpret_cast<const float4 *>(u + j * pitch + 8 * i)[1];
+                sum[j] = fma2(make_float2(f.x, f.y), w0, sum[j]);
+                sum[j] = fma2(make_float2(f.z, f.w), w1, sum[j]);
+                sum[j] = fma2(make_float2(e.x, e.y), w2, sum[j]);
+                sum[j] = fma2(make_float2(e.z, e.w), w3, sum[j]);
+            }
+        }
+        // a row without an adapter has no u: what its place held is not its sum
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j * 128] = s[j] >= 0 ? sum[j].x + sum[j].y : 0.0f;
+        return;
+    }
     for (int r = 0; r < rank; r += 32) {
         uint4 b[4][4];
 #pragma unroll
@@ -787,7 +824,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             if (col0 + n < g.N) {
 #pragma unroll 1
                 for (int j = half; j < half + 8; j += 4)
-                    four_rows<T>(g, *reinterpret_cast<const int4 *>(id + j), u + j * g.u_pitch, g.u_pitch, col0 + n, d + j * 128 + n);
+                    four_rows<T, WAVES>(g, *reinterpret_cast<const int4 *>(id + j), u + j * g.u_pitch, g.u_pitch, col0 + n, d + j * 128 + n);
             }
             __syncwarp();
             if (lane == 0) {
@@ -910,10 +947,10 @@ cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
 }
 
 // CTAs that may share a tile, one more for stretches that do not start at a tile.
-int most_parts(int64_t units, int64_t kblocks, int64_t groups) {
+int most_parts(int64_t units, int64_t kblocks, int64_t groups, int64_t most = kMaxLoraParts) {
     const int64_t len = (units * kblocks + groups - 1) / groups;
     const int64_t parts = (kblocks - 1 + len - 1) / len + 1;
-    return static_cast<int>(parts < 2 ? 2 : parts > kMaxLoraParts ? kMaxLoraParts : parts);
+    return static_cast<int>(parts < 2 ? 2 : parts > most ? most : parts);
 }
 
 struct LoraLayout {
@@ -933,7 +970,8 @@ LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int rank) {
     take(kMaxCtas * 4);
     l.off_u = take(M * rank * 4);
     if (M <= kFewRows) {
-        l.parts = M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
+        // More rows make a part dearer to write and add: the stretches are then kept longer.
+        l.parts = M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2, 4) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
         l.off_o = take(l.parts * M * N * 4);
     } else {
         const int64_t blocks = (M + 255) / 256;
