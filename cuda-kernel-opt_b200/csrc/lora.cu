@@ -447,7 +447,7 @@ struct LoraWalker {
 
 // Rows with adapters of their own: one column n per lane, four rows at a time, fp32 on pairs of ranks. The rows' adapters are read 32
 // ranks at a time: 16 loads of 16 bytes (or 8 of a whole sector) in flight per lane.
-template <typename T, bool WAVES>
+template <typename T>
 __device__ __forceinline__ void four_rows(const LoraArgs &g, const int4 id, const float *u, int pitch, int n, float *d) {
     const int rank = g.rank, s[4] = {id.x, id.y, id.z, id.w};
     const bool wide = g.wide_b != 0;
@@ -460,30 +460,34 @@ __device__ __forceinline__ void four_rows(const LoraArgs &g, const int4 id, cons
         for (int j = 0; j < 4; ++j) d[j * 128] = 0.0f;
         return;
     }
-    if (WAVES && (s[0] < 0 || s[0] == one) && (s[1] < 0 || s[1] == one) && (s[2] < 0 || s[2] == one) && (s[3] < 0 || s[3] == one)) {
-        // one adapter among them, the usual case where requests bring several rows: all of its ranks in one go
+    if ((s[0] < 0 || s[0] == one) && (s[1] < 0 || s[1] == one) && (s[2] < 0 || s[2] == one) && (s[3] < 0 || s[3] == one)) {
+        // one adapter among them, the usual case where requests bring several rows: read once, 64 ranks in one go
         const uint4 *const p = reinterpret_cast<const uint4 *>(g.lora_b + (static_cast<int64_t>(one) * g.N + n) * rank);
-        uint4 b[16];
+#pragma unroll 1
+        for (int r = 0; r < rank; r += 64) {
+            uint4 b[8];
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            if (8 * i >= rank) break;
-            if (wide) ld_32(p + i, b[i], b[i + 1]);
-            else {
-                b[i] = __ldcg(p + i);
-                b[i + 1] = 8 * i + 8 < rank ? __ldcg(p + i + 1) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8; i += 2) {
+                if (r + 8 * i >= rank) break;
+                if (wide) ld_32(p + r / 8 + i, b[i], b[i + 1]);
+                else {
+                    b[i] = __ldcg(p + r / 8 + i);
+                    b[i + 1] = r + 8 * i + 8 < rank ? __ldcg(p + r / 8 + i + 1) : make_uint4(0, 0, 0, 0);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (8 * i >= rank) break;
-            const float2 w0 = T::unpack(b[i].x), w1 = T::unpack(b[i].y), w2 = T::unpack(b[i].z), w3 = T::unpack(b[i].w);
+            for (int i = 0; i < 8; ++i) {
+                if (r + 8 * i >= rank) break;
+                const float2 w0 = T::unpack(b[i].x), w1 = T::unpack(b[i].y), w2 = T::unpack(b[i].z), w3 = T::unpack(b[i].w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 f = reinterpret_cast<const float4 *>(u + j * pitch + 8 * i)[0], e = reinterpret_cast<const float4 *>(u + j * pitch + 8 * i)[1];
-                sum[j] = fma2(make_float2(f.x, f.y), w0, sum[j]);
-                sum[j] = fma2(make_float2(f.z, f.w), w1, sum[j]);
-                sum[j] = fma2(make_float2(e.x, e.y), w2, sum[j]);
-                sum[j] = fma2(make_float2(e.z, e.w), w3, sum[j]);
+                for (int j = 0; j < 4; ++j) {
+                    const float4 *const uj = reinterpret_cast<const float4 *>(u + j * pitch + r + 8 * i);
+                    const float4 f = uj[0], e = uj[1];
+                    sum[j] = fma2(make_float2(f.x, f.y), w0, sum[j]);
+                    sum[j] = fma2(make_float2(f.z, f.w), w1, sum[j]);
+                    sum[j] = fma2(make_float2(e.x, e.y), w2, sum[j]);
+                    sum[j] = fma2(make_float2(e.z, e.w), w3, sum[j]);
+                }
             }
         }
         // a row without an adapter has no u: what its place held is not its sum
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             if (col0 + n < g.N) {
 #pragma unroll 1
                 for (int j = half; j < half + 8; j += 4)
-                    four_rows<T, WAVES>(g, *reinterpret_cast<const int4 *>(id + j), u + j * g.u_pitch, g.u_pitch, col0 + n, d + j * 128 + n);
+                    four_rows<T>(g, *reinterpret_cast<const int4 *>(id + j), u + j * g.u_pitch, g.u_pitch, col0 + n, d + j * 128 + n);
             }
             __syncwarp();
             if (lane == 0) {
