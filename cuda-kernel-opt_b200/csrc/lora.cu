@@ -1,26 +1,29 @@
 // A projection shared by all rows with low-rank adapters of many requests beside it:
 //
-//     D[i] = A[i] B^T + scale[s] (A[i] lora_a[s]^T) lora_b[s]^T,   s = row_adapter[i]
+//     D[i] = A[i] B^T + u[i] lora_b[s]^T,   u[i] = scale[s] (A[i] lora_a[s]^T),   s = row_adapter[i]
 //
-//   lora_shrink_*_kernel  u[i] = scale[s] (A[i] lora_a[s]^T), fp32, to the workspace
-//   lora_product_kernel   the shared product on tcgen05 with B's rows on the 128-row side (D is computed transposed: a lane of
-//                         tensor memory is a column of D, a column of tensor memory a row). Eight warps beside the
-//                         pipeline compute (u lora_b[s]^T)[i][n] in fp32 while the tensor core is busy and hand it to
-//                         the draining warps in pieces of 8 rows x 128 columns, which add it before the one rounding.
+// The product kernel has B's rows on the 128-row side of tcgen05.mma (D is computed transposed: a lane of tensor memory is a column
+// of D, a column of tensor memory a row). Warps beside the pipeline compute u lora_b[s]^T in fp32 while the tensor core is
+// busy ("delta warps") and hand it to the draining warps in pieces of 16 rows x 128 columns, which add it before the one
+// rounding to 16 bits.
 //
-// The adapters' second product stays off the tensor core: a zero that stands for "not this row's adapter" does not mask an
-// infinity or a NaN among an adapter's weights, so a row would see other requests' adapters; and a decode step in
-// which every row has another adapter would feed it one useful row at a time. The fp32 units have the time: rows x N x rank
-// multiply-adds against rows x N x K on the tensor core.
+// Why not on the tensor core, as further columns of K: the zero that stands for "not this row's adapter" does not mask an infinity
+// or a NaN among an adapter's weights, so a request would see other requests' adapters; and a decode step in which every
+// row has another adapter would feed it one useful row at a time. Only where 32 rows in a row have one adapter, as in a
+// prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder).
 //
-// Two forms of the product kernel, by the number of rows:
-//   one CTA, up to 256 rows    B is read once and bounds it. The K blocks of all tiles (128 columns of D, all rows) are cut
-//                              into one equal stretch per CTA (Cut); a tile that spans several CTAs leaves parts in the
-//                              workspace, and the last of its CTAs to finish adds them in ascending order. No CTA waits
-//                              for another.
-//   CTA pair, more rows        256 x 256 tiles, the tensor core bounds it: whole tiles, dealt out in waves that share
-//                              operand panels in L2, with K walked to and fro.
-// The shrink kernel lets the product start at once; only the warps that need u wait for it.
+// Three forms, by the number of rows:
+//   up to 64      one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s.
+//   65 - 256      a CTA pair per tile of 256 columns: each CTA fetches half of the rows of A for both, which at 128 rows saves a
+//                 quarter of what crosses from L2 to the SMs (192 -> 153 us at 128 x 28672 x 8192, rank 32; 125 now).
+//   more          a pair per 256 x 256 tile, whole tiles in waves, the tensor core bounds it: 4096 x 8192 x 8192, rank 64, eight
+//                 prompts, takes 400 us, 1.40 PFLOP/s, the rate that the power limit leaves a plain product.
+// In the first two the K blocks of all tiles are cut into one equal stretch per CTA or pair (Cut), so that every SM streams all the time; a
+// tile that spans several leaves parts in the workspace, and the last of its CTAs to finish adds them in ascending order. No
+// CTA waits for another, nothing is added atomically.
+//
+// u comes first, from lora_shrink_dot_kernel (up to 256 rows) or lora_list_kernel, lora_shrink_kernel and lora_join_kernel. They let the
+// product start before they are done; only its warps that need u wait.
 #include <cuda_runtime.h>
 
 #include "../../include/b200_gemm.h"
@@ -36,6 +39,7 @@ constexpr int kDeltaWarps = 8;
 constexpr int kLoraThreads = (2 + 4 + kDeltaWarps + 1) * 32;
 constexpr int kChunkRows = 16;                             // rows of D in a piece of the adapters' product
 constexpr int kChunks = 8;                                 // pieces on their way to the draining warps
+constexpr int kWaveChunks = 4;                             // the same in waves, whose ring needs the room (4096 x 8192 x 8192: 3 % over eight)
 constexpr int kAhead = 4;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
 constexpr int kOneCtaRows = 64;                            // most rows of the one-CTA form
@@ -600,6 +604,7 @@ struct PieceWalker {
 
 template <typename T, int CG, bool WAVES>
 __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __grid_constant__ LoraArgs g) {
+    constexpr int kSlots = WAVES ? kWaveChunks : kChunks;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -773,7 +778,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                         v[j] = __float_as_uint(__uint_as_float(v[j]) + delta[(slot * kChunkRows + j) * 128 + r]);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(delta_empty0 + 8 * slot);
-                    if (++slot == kChunks) slot = 0, slot_ph ^= 1u;
+                    if (++slot == kSlots) slot = 0, slot_ph ^= 1u;
                 }
                 if (mine) {
                     const int64_t row = s.m0 + c * kChunkRows;
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 mbar_arrive(delta_full0 + 8 * slot);
             }
             if (++from == kAhead) from = 0, from_ph ^= 1u;
-            if (++slot == kChunks) slot = 0, slot_ph ^= 1u;
+            if (++slot == kSlots) slot = 0, slot_ph ^= 1u;
         }
     } else {
         // -------------------------------------------------------------- u and the rows' adapters for the warps above
@@ -1071,11 +1076,11 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
     g.a_bytes = box_a * 128;
     g.u_pitch = rank + 4;   // rows of u start 16 bytes further each, modulo the banks
-        const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, rest = kChunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
+        const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, chunks = M > kFewRows ? kWaveChunks : kChunks, rest = chunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
     g.stages = (kSmemLimit - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
-    g.off_u = g.off_delta + kChunks * kChunkBytes;
+    g.off_u = g.off_delta + chunks * kChunkBytes;
     g.off_ids = g.off_u + u_bytes;
     g.off_bars = g.off_ids + kAhead * kChunkRows * 4;
     g.off_misc = g.off_bars + kLoraBars * 8;
