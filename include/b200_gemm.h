@@ -333,7 +333,10 @@ int b200_moe(int dtype, const void *X, const float *logits, const void *W13, con
  * {code, block, barrier id, phase}. Clears the record. Barrier ids of the GEMM kernel: 100 + stage a producer's
  * wait for a free stage, 300 + slot the MMA thread's wait for a drained accumulator (301 with the tall pair: the
  * lower atom's columns), 400 / 500 + stage its waits for operand data, 600 + slot a draining warp's wait for a
- * finished accumulator, 700 - 703 the cluster reduce, 800 + warp the tail split's fix-up. */
+ * finished accumulator, 700 - 703 the cluster reduce, 800 + warp the tail split's fix-up. b200_moe: 1000 + stage the weights' producer,
+ * 1100 + slot and 1200 + stage the MMA thread, 1300 + slot the draining warps, 1400 + stage the loader warps; b200_gemm_lora: 2000 - 2399
+ * the same roles, 2400 + slot and 2500 + slot the pieces of the adapters' product, 2600 and 2700 + slot their inputs, 3000 - 3399 the
+ * first product of many rows. */
 int b200_device_status(void *stream, int info[4]);
 /* Test hook: the budget of every in-kernel wait, in nanoseconds (default 2e9). */
 void b200_set_wait_budget_ns(uint64_t ns);
