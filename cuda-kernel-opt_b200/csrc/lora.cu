@@ -12,18 +12,19 @@
 // row has another adapter would feed it one useful row at a time. Only where 32 rows in a row have one adapter, as in a
 // prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder).
 //
-// Three forms, by the number of rows:
-//   up to 64      one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s.
-//   65 - 256      a CTA pair per tile of 256 columns: each CTA fetches half of the rows of A for both, which at 128 rows saves a
-//                 quarter of what crosses from L2 to the SMs (192 -> 153 us at 128 x 28672 x 8192, rank 32; 125 now).
-//   more          a pair per 256 x 256 tile, whole tiles in waves, the tensor core bounds it: 4096 x 8192 x 8192, rank 64, eight
-//                 prompts, takes 400 us, 1.40 PFLOP/s, the rate that the power limit leaves a plain product.
-// In the first two the K blocks of all tiles are cut into one equal stretch per CTA or pair (Cut), so that every SM streams all the time; a
-// tile that spans several leaves parts in the workspace, and the last of its CTAs to finish adds them in ascending order. No
-// CTA waits for another, nothing is added atomically.
+// Two forms, by the number of rows:
+//   up to 256     one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s; 128
+//                 rows, rank 32, any of 64 adapters per row, 126 us, 4.8 TB/s. The K blocks of all tiles are cut into one equal
+//                 stretch per CTA (Cut), so that every SM streams all the time; a tile that spans several leaves parts in the
+//                 workspace, and the last of its CTAs to finish adds them in ascending order. No CTA waits for another,
+//                 nothing is added atomically. (A CTA pair per 256 columns, which halves what the rows of A cost between L2 and
+//                 SMs, measured the same within 1 % from 65 to 256 rows.)
+//   more          a CTA pair per 256 x 256 tile, whole tiles in waves, the tensor core bounds it: 4096 x 8192 x 8192, rank 64, eight
+//                 prompts, takes 400 us, 1.40 PFLOP/s, the rate that the power limit leaves a plain product. 512 rows take 66 us,
+//                 two calls of 256 rows 196.
 //
-// u comes first, from lora_shrink_dot_kernel (up to 256 rows) or lora_list_kernel, lora_shrink_kernel and lora_join_kernel. They let the
-// product start before they are done; only its warps that need u wait.
+// u comes first, from lora_shrink_dot_kernel (few rows) or lora_list_kernel, lora_shrink_kernel and lora_join_kernel. They let the product
+// start before they are done; only its warps that need u wait.
 #include <cuda_runtime.h>
 
 #include "../../include/b200_gemm.h"
@@ -42,8 +43,7 @@ constexpr int kChunks = 8;                                 // pieces on their wa
 constexpr int kWaveChunks = 4;                             // the same in waves, whose ring needs the room (4096 x 8192 x 8192: 3 % over eight)
 constexpr int kAhead = 4;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
-constexpr int kOneCtaRows = 64;                            // most rows of the one-CTA form
-constexpr int kFewRows = 256;                              // most rows that one tile takes
+constexpr int kFewRows = 256;                              // most rows of the one-CTA form
 constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kChunks + 2 * kAhead;
 constexpr int kNoRow = -2;                                 // in the place of an adapter: behind the last row
 constexpr int kMaxLoraParts = 16;
@@ -55,7 +55,7 @@ constexpr int kGroupRows = 16;                             // pair: row blocks t
 
 struct alignas(64) LoraArgs {
     CUtensorMap map_b, map_a;      // B as {K, N}, A as {K, M}
-    CUtensorMap map_la, map_lb, map_u;   // many rows: lora_a as {K, adapters * rank}, lora_b as {rank, adapters * N}, u16 as {rank, 2 * M}
+    CUtensorMap map_s, map_la, map_lb, map_u;   // listed: A in boxes of 128 rows, lora_a as {K, adapters * rank}; many rows: lora_b as {rank, adapters * N}, u16 as {rank, 2 * M}
     const uint16_t *A, *lora_a, *lora_b;
     uint16_t *D;
     const float *scale;
@@ -67,7 +67,8 @@ struct alignas(64) LoraArgs {
         int *count, *adapter, *entry;   // per block of 256 rows: adapters that occur, and which; per row: which of them it has
         int *wide;                 // per 32 rows: some u does not fit a pair of 16-bit numbers
     } list;
-    int parts_u, on_tensor;        // parts of u; whether the adapters' second product may use the tensor core
+    int waves;                     // the form of the product: its own parameter, the last pass of many rows may be short
+    int listed, parts_u, on_tensor;   // u by lists of adapters; its parts; whether the adapters' second product may use the tensor core
     uint32_t idesc_u, idesc_run;   // run: with N = 0
     float *o;                      // [part][M][N]: sums of tiles that span CTAs
     int *arrived;                  // per CTA: the warps that are done with the tile it began last
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(256) lora_list_kernel(const __grid_constant__ 
     griddep_launch_dependents();
     const int i = threadIdx.x, m = blockIdx.x * 256 + i, warp = i >> 5, lane = i & 31;
     const int id = row_adapter(g, m);
+    if (blockIdx.x == 0) g.arrived[i] = 0;                 // kMaxCtas of them
     // one row of the warp per adapter leads; it looks for its adapter among the leaders of the warps before
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     const int leader = __ffs(same) - 1;
@@ -275,8 +277,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_kernel(const __
                 if (issuer) {
                     mbar_arrive_expect_tx(bar, (g.rank + 256) * 128);
                     tma_load_2d(dst, &g.map_la, bar, kb * 64, row);
-                    tma_load_2d_hint(dst + 128 * 128, &g.map_a, bar, kb * 64, block * 256, keep);
-                    tma_load_2d_hint(dst + 256 * 128, &g.map_a, bar, kb * 64, block * 256 + 128, keep);
+                    tma_load_2d_hint(dst + 128 * 128, &g.map_s, bar, kb * 64, block * 256, keep);
+                    tma_load_2d_hint(dst + 256 * 128, &g.map_s, bar, kb * 64, block * 256 + 128, keep);
                 }
                 if (++st == kShrinkStages) st = 0, ph ^= 1u;
             }
@@ -384,11 +386,13 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
             fits = fits && fabsf(f[j]) <= T::kMax;
         }
         *reinterpret_cast<float4 *>(g.u + static_cast<int64_t>(m) * g.rank + r) = make_float4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<uint2 *>(g.u16 + static_cast<int64_t>(m) * g.rank + r) = make_uint2(hi[0] | static_cast<uint32_t>(hi[1]) << 16, hi[2] | static_cast<uint32_t>(hi[3]) << 16);
-        *reinterpret_cast<uint2 *>(g.u16 + (static_cast<int64_t>(g.M) + m) * g.rank + r) = make_uint2(lo[0] | static_cast<uint32_t>(lo[1]) << 16, lo[2] | static_cast<uint32_t>(lo[3]) << 16);
+        if (g.waves) {
+            *reinterpret_cast<uint2 *>(g.u16 + static_cast<int64_t>(m) * g.rank + r) = make_uint2(hi[0] | static_cast<uint32_t>(hi[1]) << 16, hi[2] | static_cast<uint32_t>(hi[3]) << 16);
+            *reinterpret_cast<uint2 *>(g.u16 + (static_cast<int64_t>(g.M) + m) * g.rank + r) = make_uint2(lo[0] | static_cast<uint32_t>(lo[1]) << 16, lo[2] | static_cast<uint32_t>(lo[3]) << 16);
+        }
     }
     const int all = __syncthreads_and(fits);
-    if (threadIdx.x == 0) g.list.wide[blockIdx.x] = !all;
+    if (g.waves && threadIdx.x == 0) g.list.wide[blockIdx.x] = !all;
 }
 
 // ---------------------------------------------------------------------------------------------- shared product
@@ -399,8 +403,9 @@ struct LoraSegment {
     int own0, own1, row0, row1;    // few rows: the pieces that this part adds; where there is one piece, its rows / 4
 };
 
-template <int CG, bool WAVES>
+template <bool WAVES>
 struct LoraWalker {
+    static constexpr int CG = WAVES ? 2 : 1;
     int q, end, step, tiles_n, row_blocks, kblocks, rows, m, group;   // group: a CTA or a pair
     Cut cut;
     __device__ __forceinline__ LoraWalker(const LoraArgs &g)
@@ -582,13 +587,13 @@ __device__ __forceinline__ bool has_piece(const LoraSegment &s, const Groups &v,
 }
 
 // The pieces of one CTA in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
-template <int CG, bool WAVES>
+template <bool WAVES>
 struct PieceWalker {
-    LoraWalker<CG, WAVES> walk;
+    LoraWalker<WAVES> walk;
     LoraSegment s;
     Groups v;
     int c, rows;
-    __device__ __forceinline__ PieceWalker(const LoraWalker<CG, WAVES> &w) : walk(w) { c = rows = 0; }
+    __device__ __forceinline__ PieceWalker(const LoraWalker<WAVES> &w) : walk(w) { c = rows = 0; }
     __device__ __forceinline__ bool next(const LoraArgs &g, int lane) {
         ++c;
         for (;; ++c) {
@@ -603,9 +608,9 @@ struct PieceWalker {
     }
 };
 
-template <typename T, int CG, bool WAVES>
+template <typename T, bool WAVES>
 __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __grid_constant__ LoraArgs g) {
-    constexpr int kSlots = WAVES ? kWaveChunks : kChunks;
+    constexpr int CG = WAVES ? 2 : 1, kSlots = WAVES ? kWaveChunks : kChunks;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -650,7 +655,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     constexpr int kBBytes = 128 * 128;                     // 128 rows of B, 64 elements of K
     const uint32_t stage_bytes = kBBytes + g.a_bytes;
     const int stages = g.stages;
-    LoraWalker<CG, WAVES> walk(g);
+    LoraWalker<WAVES> walk(g);
     LoraSegment s;
     int st = 0;
     uint32_t ph = 0;
@@ -809,7 +814,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 // two tiles that it does not finish); the CTA whose warp is the last one adds the parts in the end.
                 __threadfence();
                 __syncwarp();
-                if (lane == 0 && atomicAdd(g.arrived + blockIdx.x - CG * s.part, 1) == 4 * s.parts - 1) {
+                if (lane == 0 && atomicAdd(g.arrived + blockIdx.x - s.part, 1) == 4 * s.parts - 1) {
                     __threadfence();
                     misc[s.kb0 > 0 ? 2 : 3] = s.tile;
                 }
@@ -820,7 +825,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         const int w = warp - 6, n = (w & 3) * 32 + lane, half = (w >> 2) * 8;
         int slot = 0, from = 0;
         uint32_t slot_ph = 1, from_ph = 0;
-        PieceWalker<CG, WAVES> at(walk);
+        PieceWalker<WAVES> at(walk);
         griddep_wait();                                    // nothing that this SM's first-level cache may hold is older than the operands
         while (ok && at.next(g, lane)) {
             const int col0 = (at.s.tile * CG + static_cast<int>(rank)) * 128;
@@ -846,7 +851,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         }
     } else {
         // -------------------------------------------------------------- u and the rows' adapters for the warps above
-        PieceWalker<CG, WAVES> at(walk);
+        PieceWalker<WAVES> at(walk);
         int from = 0;
         uint32_t ph_from = 1;
         griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         for (int i = 2; i < 4; ++i) {
             const int tile = misc[i];
             if (tile < 0) continue;
-            const int parts = walk.cut.num_parts(tile), col = (tile * CG + static_cast<int>(rank)) * 128 + lane * 4;
+            const int parts = walk.cut.num_parts(tile), col = tile * 128 + lane * 4;
             if (col >= g.N) continue;
             const int64_t pitch = static_cast<int64_t>(g.M) * g.N;
             constexpr int kWarps = kLoraThreads / 32;
@@ -942,7 +947,7 @@ cudaError_t launch(Kernel *kernel, const LoraArgs &g, dim3 grid, int threads, in
 template <typename T>
 cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
     cudaError_t e;
-    if (g.M <= kFewRows) {
+    if (!g.listed) {
         const int blocks = g.M * (g.rank / 4);
         e = launch(lora_shrink_dot_kernel<T>, g, blocks < 8 * g.sms ? blocks : 8 * g.sms, 256, 0, 1, stream);
     } else {
@@ -951,9 +956,8 @@ cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
         if (e == cudaSuccess) e = launch(lora_join_kernel<T>, g, (g.M + 31) / 32, 32 * (g.rank / 4), 0, 1, stream);
     }
     if (e != cudaSuccess) return e;
-    if (g.M <= kOneCtaRows) return launch(lora_product_kernel<T, 1, false>, g, g.sms, kLoraThreads, smem, 1, stream);
-    if (g.M <= kFewRows) return launch(lora_product_kernel<T, 2, false>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
-    return launch(lora_product_kernel<T, 2, true>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
+    if (!g.waves) return launch(lora_product_kernel<T, false>, g, g.sms, kLoraThreads, smem, 1, stream);
+    return launch(lora_product_kernel<T, true>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
 }
 
 // CTAs that may share a tile, one more for stretches that do not start at a tile.
@@ -964,11 +968,12 @@ int most_parts(int64_t units, int64_t kblocks, int64_t groups, int64_t most = kM
 }
 
 struct LoraLayout {
+    bool listed;
     int parts, parts_u;
     int64_t off_u, off_o, off_u16, off_u_parts, off_count, off_adapter, off_entry, off_wide, bytes;
 };
 
-LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int rank) {
+LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) {
     LoraLayout l = {};
     if (M > kMaxBlocks * 256) M = kMaxBlocks * 256;
     int64_t at = 0;
@@ -980,19 +985,26 @@ LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int rank) {
     take(kMaxCtas * 4);
     l.off_u = take(M * rank * 4);
     if (M <= kFewRows) {
-        // More rows make a part dearer to write and add: the stretches are then kept longer.
-        l.parts = M > kOneCtaRows ? most_parts((N + 255) / 256, (K + 63) / 64, kLoraGridSms / 2, 4) : most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms);
+        // More rows make a part dearer to write and add, the stretches are then kept longer (77 x 4104 x 2056: 16.2 us with
+        // four parts, 22.9 with six).
+        l.parts = most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms, M > 64 ? 4 : kMaxLoraParts);
         l.off_o = take(l.parts * M * N * 4);
     } else {
-        const int64_t blocks = (M + 255) / 256;
         l.parts = 2;
-        l.parts_u = most_parts(blocks, (K + 63) / 64, kLoraGridSms);
         l.off_u16 = take(2 * M * rank * 2);
+        l.off_wide = take((M + 31) / 32 * 4);
+    }
+    // Up to 256 rows u comes by dot products, which read an adapter for each of its rows, unless that is much more than the products by
+    // lists read, which read the rows for each adapter, and enough to pay for two more kernels (256 x 8192 x 8192, rank 64, four
+    // adapters: 73 -> 60 us).
+    l.listed = M > kFewRows || (M * rank > 2 * (num_adapters < M ? num_adapters : M) * (256 + rank) && M * rank * K * 2 > (int64_t(64) << 20));
+    if (l.listed) {
+        const int64_t blocks = (M + 255) / 256;
+        l.parts_u = most_parts(blocks, (K + 63) / 64, kLoraGridSms);
         l.off_u_parts = take(l.parts_u * M * rank * 4);
         l.off_count = take(blocks * 4);
         l.off_adapter = take(blocks * 256 * 4);
         l.off_entry = take(M * 4);
-        l.off_wide = take((M + 31) / 32 * 4);
     }
     l.bytes = at;
     return l;
@@ -1010,8 +1022,7 @@ int check_lora(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) 
 
 int prepare_moe_kernels();
 int prepare_routed_kernels() {
-    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, 1, false>, lora_product_kernel<Bf16, 2, false>, lora_product_kernel<Bf16, 2, true>,
-                                         lora_product_kernel<Fp16, 1, false>, lora_product_kernel<Fp16, 2, false>, lora_product_kernel<Fp16, 2, true>};
+    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, false>, lora_product_kernel<Bf16, true>, lora_product_kernel<Fp16, false>, lora_product_kernel<Fp16, true>};
     for (const auto k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
@@ -1025,7 +1036,7 @@ int prepare_routed_kernels() {
 
 extern "C" int64_t b200_gemm_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) {
     if (b200::check_lora(M, N, K, num_adapters, rank) != B200_OK) return -1;
-    return b200::lora_layout(M, N, K, rank).bytes;
+    return b200::lora_layout(M, N, K, num_adapters, rank).bytes;
 }
 
 extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D, int64_t M, int64_t N, int64_t K, const void *lora_a,
@@ -1050,7 +1061,7 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     st = current_device(&g.sms, &g.status);
     if (st != B200_OK) return st;
     if (g.sms > kMaxCtas) g.sms = kMaxCtas;
-    const LoraLayout l = lora_layout(M, N, K, rank);
+    const LoraLayout l = lora_layout(M, N, K, num_adapters, rank);
     g.lora_a = static_cast<const uint16_t *>(lora_a);
     g.lora_b = static_cast<const uint16_t *>(lora_b);
     g.scale = lora_scale;
@@ -1070,8 +1081,10 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.num_adapters = static_cast<int>(num_adapters);
     g.parts = l.parts;
     g.parts_u = l.parts_u;
+    g.listed = l.listed;
+    g.waves = M > kFewRows;
     const bool bf16 = dtype == B200_BF16;
-    const int cg = M > kOneCtaRows ? 2 : 1;
+    const int cg = M > kFewRows ? 2 : 1;
     g.rows = M > kFewRows ? 256 : static_cast<int>((M + 16 * cg - 1) / (16 * cg) * (16 * cg));
     const int box_a = g.rows / cg;
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
@@ -1092,10 +1105,10 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.idesc_u = umma_idesc(128, 256, bf16);
     g.budget = wait_budget_cycles();
     st = encode_operand_map(&g.map_b, dtype, Bt, K, N, 128);
+    if (st == B200_OK && l.listed) st = encode_operand_map(&g.map_la, dtype, lora_a, K, num_adapters * rank, rank);
     if (st == B200_OK && M > kFewRows) {
         g.on_tensor = num_adapters * N < (int64_t(1) << 31) - 512;   // rows of lora_b as the copies count them
-        st = encode_operand_map(&g.map_la, dtype, lora_a, K, num_adapters * rank, rank);
-        if (st == B200_OK && g.on_tensor) st = encode_operand_map(&g.map_lb, dtype, lora_b, rank, num_adapters * N, 128);
+        if (g.on_tensor) st = encode_operand_map(&g.map_lb, dtype, lora_b, rank, num_adapters * N, 128);
     }
     for (int64_t m0 = 0; st == B200_OK && m0 < M; m0 += kMaxBlocks * 256) {
         const int64_t rows = M - m0 < kMaxBlocks * 256 ? M - m0 : kMaxBlocks * 256;
@@ -1104,6 +1117,7 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
         g.row_adapter = row_adapter + m0;
         g.M = static_cast<int>(rows);
         st = encode_operand_map(&g.map_a, dtype, g.A, K, rows, box_a);
+        if (st == B200_OK && l.listed) st = encode_operand_map(&g.map_s, dtype, g.A, K, rows, 128);
         if (st == B200_OK && M > kFewRows && g.on_tensor) st = encode_operand_map(&g.map_u, dtype, g.u16, rank, 2 * rows, 128);
         if (st != B200_OK) break;
         const cudaError_t e = bf16 ? launch_lora<Bf16>(g, smem, static_cast<cudaStream_t>(stream)) : launch_lora<Fp16>(g, smem, static_cast<cudaStream_t>(stream));

@@ -479,6 +479,27 @@ def test_lora_more_rows_than_one_pass_and_offsets_past_32_bits(pkg, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [65536 + 7, 65536 + 300])
+def test_lora_a_short_last_pass(pkg, cuda, m):
+    x, w, a, b, scale = lora_inputs(cuda, "fp16", m, 72, 136, 8, 4, m)
+    ids = ((cuda.arange(m, device="cuda") // 501) % 5 - 1).to(cuda.int32)
+    got = run_lora(pkg, cuda, x, w, a, b, ids, scale)
+    check_close(got, *lora_want(cuda, x, w, a, b, ids, scale), "fp16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [150, 256])
+def test_lora_few_adapters_with_many_rows_each(pkg, cuda, m):
+    """Up to 256 rows whose first product goes by lists of adapters: a large rank, few adapters, a long K."""
+    for order in ("mixed", "stretches", "none", "all"):
+        x, w, a, b, scale = lora_inputs(cuda, "bf16", m, 392, 8200, 128, 2, m)
+        ids = lora_ids(cuda, order, m, 2, m)
+        got = run_lora(pkg, cuda, x, w, a, b, ids, scale)
+        check_close(got, *lora_want(cuda, x, w, a, b, ids, scale), "bf16")
+        assert cuda.equal(run_lora(pkg, cuda, x, w, a, b, ids, scale), got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 40])
 def test_moe_weights_past_32_bits(pkg, cuda, tokens):
     """W13 has more than 2^32 elements, W2 more than 2^31; the chosen experts lie at both ends."""
