@@ -258,7 +258,7 @@ def gemm(A, Bt, Cm=None, D=None, alpha=1.0, beta=0.0, params: Params | None = No
 
 
 _CODES = {}   # torch dtype -> B200_F16 / B200_BF16, filled on first use
-_NEEDS = {}   # sizes of a call -> bytes of its workspace
+_LORA_NEEDS, _MOE_NEEDS = {}, {}   # every size of a call -> bytes of its workspace
 
 
 def _torch():
@@ -329,11 +329,11 @@ def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, works
 def _gemm_lora(torch, code, A, Bt, lora_a, lora_b, row_adapter, lora_scale, D, workspace, M, N, K, S, R, stream):
     L = _lib or lib()
     if workspace is None:
-        need = _NEEDS.get((M, N, K, R))
+        need = _LORA_NEEDS.get((M, N, K, S, R))
         if need is None:
             need = max(L.b200_gemm_lora_workspace_bytes(M, N, K, S, R), 0)
-            if need and len(_NEEDS) < 4096:
-                _NEEDS[M, N, K, R] = need
+            if need and len(_LORA_NEEDS) < 4096:
+                _LORA_NEEDS[M, N, K, S, R] = need
         workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=A.device)   # the quickest of torch's allocations
     if D is None:
         D = torch.empty_strided((M, N), (N, 1), dtype=A.dtype, device=A.device)
@@ -383,11 +383,11 @@ def _moe(torch, code, X, logits, W13, W2, normalise, Y, ids, weights, workspace,
     L = _lib or lib()
     dev = X.device
     if workspace is None:
-        need = _NEEDS.get((T, H, I, E, k))
+        need = _MOE_NEEDS.get((T, H, I, E, k))
         if need is None:
             need = max(L.b200_moe_workspace_bytes(T, H, I, E, k), 0)
-            if need and len(_NEEDS) < 4096:
-                _NEEDS[T, H, I, E, k] = need
+            if need and len(_MOE_NEEDS) < 4096:
+                _MOE_NEEDS[T, H, I, E, k] = need
         workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)   # the quickest of torch's allocations
     if Y is None:
         Y = torch.empty_like(X)

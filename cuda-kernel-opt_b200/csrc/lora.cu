@@ -51,7 +51,7 @@ constexpr int kMaxCtas = 256;
 constexpr int kMaxBlocks = 256;                            // blocks of 256 rows of one pass; more rows are several passes
 constexpr int kGroup = 32;                                 // rows that share a way of adding their adapters
 constexpr int kLoraGridSms = 148;                          // what the workspace is sized for
-constexpr int kGroupRows = 16;                             // pair: row blocks that a wave walks together
+constexpr int kGroupRows = 16;                             // row blocks that a wave walks together
 
 struct alignas(64) LoraArgs {
     CUtensorMap map_b, map_a;      // B as {K, N}, A as {K, M}
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------------------------------------- shared product
 
-// K blocks [kb0, kb1) of the tile at row m0 and 128-column (pair: 256-column) tile `tile`, as part `part` of `parts`.
+// K blocks [kb0, kb1) of the tile at row m0 and 128-column (waves: 256-column) tile `tile`, as part `part` of `parts`.
 struct LoraSegment {
     int tile, m0, kb0, kb1, part, parts;
     int own0, own1, row0, row1;    // few rows: the pieces that this part adds; where there is one piece, its rows / 4
@@ -1084,13 +1084,14 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.listed = l.listed;
     g.waves = M > kFewRows;
     const bool bf16 = dtype == B200_BF16;
-    const int cg = M > kFewRows ? 2 : 1;
-    g.rows = M > kFewRows ? 256 : static_cast<int>((M + 16 * cg - 1) / (16 * cg) * (16 * cg));
+    const int cg = g.waves ? 2 : 1;
+    g.rows = g.waves ? 256 : static_cast<int>((M + 15) / 16 * 16);
     const int box_a = g.rows / cg;
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
     g.a_bytes = box_a * 128;
     g.u_pitch = rank + 4;   // rows of u start 16 bytes further each, modulo the banks
-        const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, chunks = M > kFewRows ? kWaveChunks : kChunks, rest = chunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
+    const int u_bytes = kAhead * kChunkRows * g.u_pitch * 4, chunks = g.waves ? kWaveChunks : kChunks;
+    const int rest = chunks * kChunkBytes + u_bytes + kAhead * kChunkRows * 4 + kLoraBars * 8 + 16;
     g.stages = (kSmemLimit - 1024 - rest) / (128 * 128 + g.a_bytes);
     if (g.stages > kLoraStages) g.stages = kLoraStages;
     g.off_delta = g.stages * (128 * 128 + g.a_bytes);
@@ -1106,7 +1107,7 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.budget = wait_budget_cycles();
     st = encode_operand_map(&g.map_b, dtype, Bt, K, N, 128);
     if (st == B200_OK && l.listed) st = encode_operand_map(&g.map_la, dtype, lora_a, K, num_adapters * rank, rank);
-    if (st == B200_OK && M > kFewRows) {
+    if (st == B200_OK && g.waves) {
         g.on_tensor = num_adapters * N < (int64_t(1) << 31) - 512;   // rows of lora_b as the copies count them
         if (g.on_tensor) st = encode_operand_map(&g.map_lb, dtype, lora_b, rank, num_adapters * N, 128);
     }
@@ -1118,7 +1119,7 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
         g.M = static_cast<int>(rows);
         st = encode_operand_map(&g.map_a, dtype, g.A, K, rows, box_a);
         if (st == B200_OK && l.listed) st = encode_operand_map(&g.map_s, dtype, g.A, K, rows, 128);
-        if (st == B200_OK && M > kFewRows && g.on_tensor) st = encode_operand_map(&g.map_u, dtype, g.u16, rank, 2 * rows, 128);
+        if (st == B200_OK && g.on_tensor) st = encode_operand_map(&g.map_u, dtype, g.u16, rank, 2 * rows, 128);
         if (st != B200_OK) break;
         const cudaError_t e = bf16 ? launch_lora<Bf16>(g, smem, static_cast<cudaStream_t>(stream)) : launch_lora<Fp16>(g, smem, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) st = record_cuda_error(e);

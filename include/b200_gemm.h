@@ -291,7 +291,10 @@ int b200_session_gemm_host_sharded(b200_session *s, int dtype, const void *hA_ro
  * outputs are fp16 or bf16 (dtype), sums are fp32, outputs are rounded once. As everywhere here the calls
  * allocate nothing, enqueue on the given stream and return; the same inputs give the same bits. The workspace
  * (256-byte aligned, any contents) holds intermediate sums: calls that may overlap on the GPU (two streams,
- * two graphs replayed side by side) need one each. Outputs must not overlap inputs or the workspace. */
+ * two graphs replayed side by side) need one each. Its size is asked for with the sizes of the call: fewer rows or
+ * adapters can need more. Outputs must not overlap inputs or the workspace. A number that is not finite reaches no row but
+ * those whose own sums hold it. There an infinity among lora_b's or W2's weights may arrive as a NaN: the number
+ * it is multiplied with can be held as two 16-bit ones. */
 
 /* A projection shared by all rows with low-rank adapters of many requests beside it:
  *

@@ -500,6 +500,17 @@ def test_lora_few_adapters_with_many_rows_each(pkg, cuda, m):
 
 
 @pytest.mark.gpu
+def test_lora_workspace_of_each_number_of_adapters(pkg, cuda):
+    """Few adapters need more workspace than many at the same sizes; the calls that allocate it themselves notice."""
+    m, n, k, r = 256, 64, 1032, 128
+    assert pkg.gemm_lora_workspace_bytes(m, n, k, 2, r) > pkg.gemm_lora_workspace_bytes(m, n, k, 256, r)
+    for s in (256, 2, 256, 2):
+        x, w, a, b, scale = lora_inputs(cuda, "bf16", m, n, k, r, s, s)
+        ids = lora_ids(cuda, "mixed", m, s, s)
+        check_close(pkg.gemm_lora(x, w, a, b, ids, scale), *lora_want(cuda, x, w, a, b, ids, scale), "bf16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 40])
 def test_moe_weights_past_32_bits(pkg, cuda, tokens):
     """W13 has more than 2^32 elements, W2 more than 2^31; the chosen experts lie at both ends."""
