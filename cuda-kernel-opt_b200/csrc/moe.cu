@@ -28,7 +28,7 @@
 //
 // All are launched as programmatic dependents: DOWN_FEW starts as soon as UP_FEW runs (two CTAs fit an SM), fills its ring with weights and
 // waits only before it reads UP's sums. Measured as device time in a graph: 16 tokens, 64 experts of 4096 x 2048, top 6, 397 us:
-// 6.4 TB/s, 98 % of the copy rate; 64 tokens, experts of 4096 x 1408, 350 us, 96 %; 256 tokens as above 229 us, 80 %: the
+// 6.4 TB/s, 98 % of the copy rate; 64 tokens, experts of 4096 x 1408, 350 us, 96 %; 256 tokens as above 228 us, 81 %: the
 // activations and sums of 2048 slots cross the L2 beside the weights; one token, 8 of 128 experts of 2048 x 768, 28 us, 40 %:
 // the choice, two starts and two joins of some microseconds each frame 11 us of reading.
 #include <cuda_runtime.h>
@@ -298,22 +298,22 @@ enum Product {
                // of Y adds the tile's parts
 };
 
-// The gated value of four neighbouring inner rows of one slot from UP's parts (ascending, four of them in flight), as pairs of
+// The gated value of four neighbouring inner rows of one slot from UP's parts (ascending, BATCH of them in flight), as pairs of
 // 16-bit numbers. The exponential and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th
 // of an fp16.
-template <typename T>
+template <typename T, int BATCH>
 __device__ __forceinline__ void gated_values(const float *z, int inner, int parts, int64_t part_pitch, uint2 &hi, uint2 &lo) {
     float4 gate = make_float4(0.0f, 0.0f, 0.0f, 0.0f), up = gate;
-    for (int p0 = 0; p0 < parts; p0 += 4, z += 4 * part_pitch) {
-        float4 a[4], b[4];
+    for (int p0 = 0; p0 < parts; p0 += BATCH, z += BATCH * part_pitch) {
+        float4 a[BATCH], b[BATCH];
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
+        for (int p = 0; p < BATCH; ++p)
             if (p0 + p < parts) {
                 a[p] = __ldcg(reinterpret_cast<const float4 *>(z + p * part_pitch));
                 b[p] = __ldcg(reinterpret_cast<const float4 *>(z + p * part_pitch + inner));
             }
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
+        for (int p = 0; p < BATCH; ++p)
             if (p0 + p < parts) {
                 gate.x += a[p].x, gate.y += a[p].y, gate.z += a[p].z, gate.w += a[p].w;
                 up.x += b[p].x, up.y += b[p].y, up.z += b[p].z, up.w += b[p].w;
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                         const int parts = up.num_parts(s.ai * tiles_up + kb), k4 = kb * 64 + (lane & 15) * 4;
                         for (int r = row0; r < count; r += row_step) {
                             uint2 hi = make_uint2(0, 0), lo = hi;
-                            if (k4 < g.inner) gated_values<T>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k4, g.inner, parts, part_pitch, hi, lo);
+                            if (k4 < g.inner) gated_values<T, 4>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k4, g.inner, parts, part_pitch, hi, lo);
                             const uint32_t at = dst + swizzled(r, (lane & 15) >> 1) + (lane & 1) * 8;
                             st_shared_v2(at, hi);
                             st_shared_v2(at + rows_bytes, lo);
@@ -718,7 +718,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     }
 }
 
-// The gated values for DOWN: four inner rows of one slot per thread.
+// The gated values for DOWN: four inner rows of one slot per thread. Where it has much to do a slot's values come in one or two parts, so
+// more threads per SM serve better than more parts in flight (256 tokens, 128 experts of 2048 x 768, top 8: 232 us for
+// the layer with four, 228 with two; 129 tokens, 7 experts of 1560 x 248, many parts: 37 against 38).
 template <typename T>
 __global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
     griddep_launch_dependents();   // DOWN reads nothing of this kernel before its own wait
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ M
     const int atoms = tile_atoms(g, most), tiles = ((g.inner + 63) / 64 + atoms - 1) / atoms;
     const Cut up(chosen * tiles, (g.hidden + 63) / 64, g.sms, g.parts_up);
     uint2 hi, lo;
-    gated_values<T>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(owner * tiles + k / 64 / atoms),
+    gated_values<T, 2>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(owner * tiles + k / 64 / atoms),
                     static_cast<int64_t>(g.slots) * 2 * g.inner, hi, lo);
     *reinterpret_cast<uint2 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = hi;
     *reinterpret_cast<uint2 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = lo;
