@@ -12,13 +12,18 @@
 // row has another adapter would feed it one useful row at a time. Only where 32 rows in a row have one adapter, as in a
 // prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder).
 //
-// Two forms, by the number of rows:
+// Three forms, by the numbers of rows and columns:
 //   up to 256     one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s; 128
 //                 rows, rank 32, any of 64 adapters per row, 126 us, 4.8 TB/s. The K blocks of all tiles are cut into one equal
 //                 stretch per CTA (Cut), so that every SM streams all the time; a tile that spans several leaves parts in the
 //                 workspace, and the last of its CTAs to finish adds them in ascending order. No CTA waits for another,
 //                 nothing is added atomically. (A CTA pair per 256 columns, which halves what the rows of A cost between L2 and
 //                 SMs, measured the same within 1 % from 65 to 256 rows.)
+//   few columns   the same with the rows in several blocks, each with its own stretches: more CTAs share the work, the rows' adapters
+//                 above all. 225 x 672 x 3120, rank 72, any of 14 adapters per row: 107 -> 48 us, 25 x 384 x 744, rank 120: 39 ->
+//                 19.5; beyond 256 rows while waves would have at most 18 tiles: 535 x 312 x 360, rank 72, 43 prompts: 134 ->
+//                 39 us against waves, 1024 x 2048 x 2048 (32 tiles): 30 in waves, 45 in blocks. A kernel of its own, the
+//                 general walk costs the form above 5 % of its smallest calls.
 //   more          a CTA pair per 256 x 256 tile, whole tiles in waves, the tensor core bounds it: 4096 x 8192 x 8192, rank 64, eight
 //                 prompts, takes 400 us, 1.40 PFLOP/s, the rate that the power limit leaves a plain product. 512 rows of eight
 //                 prompts take 78 us, two calls of 256 rows 125.
@@ -43,7 +48,7 @@ constexpr int kChunks = 8;                                 // pieces on their wa
 constexpr int kWaveChunks = 4;                             // the same in waves, whose ring needs the room (4096 x 8192 x 8192: 3 % over eight)
 constexpr int kAhead = 4;                                  // pieces whose adapters and u are on their way to the delta warps
 constexpr int kChunkBytes = kChunkRows * 128 * 4;
-constexpr int kFewRows = 256;                              // most rows of the one-CTA form
+constexpr int kTileRows = 256;                             // most rows of a tile
 constexpr int kLoraBars = 2 * kLoraStages + 4 + 2 * kChunks + 2 * kAhead;
 constexpr int kNoRow = -2;                                 // in the place of an adapter: behind the last row
 constexpr int kMaxLoraParts = 16;
@@ -400,41 +405,45 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
 // K blocks [kb0, kb1) of the tile at row m0 and 128-column (waves: 256-column) tile `tile`, as part `part` of `parts`.
 struct LoraSegment {
     int tile, m0, kb0, kb1, part, parts;
-    int own0, own1, row0, row1;    // few rows: the pieces that this part adds; where there is one piece, its rows / 4
+    int unit, own0, own1, row0, row1;   // stretches: number of the tile; the pieces that this part adds; their rows / 4, all but where there is one piece
 };
 
-template <bool WAVES>
+enum Form { ONE, BLOCKS, WAVES };   // stretches with all rows in a tile; stretches with several blocks of rows; waves of whole tiles
+
+template <Form F>
 struct LoraWalker {
-    static constexpr int CG = WAVES ? 2 : 1;
-    int q, end, step, tiles_n, row_blocks, kblocks, rows, m, group;   // group: a CTA or a pair
+    static constexpr int CG = F == WAVES ? 2 : 1;
+    int q, end, tiles_n, row_blocks;
     Cut cut;
     __device__ __forceinline__ LoraWalker(const LoraArgs &g)
-        : tiles_n((g.N + 128 * CG - 1) / (128 * CG)), row_blocks((g.M + g.rows - 1) / g.rows), kblocks((g.K + 63) / 64), rows(g.rows), m(g.M),
-          group(blockIdx.x / CG), cut(WAVES ? 0 : tiles_n, kblocks, gridDim.x / CG, g.parts) {
-        if (WAVES) {
-            q = group;
-            step = gridDim.x / CG;
+        : tiles_n((g.N + 128 * CG - 1) / (128 * CG)), row_blocks(F == ONE ? 1 : (g.M + g.rows - 1) / g.rows), cut(F == WAVES ? 0 : tiles_n * row_blocks, (g.K + 63) / 64, gridDim.x, g.parts) {
+        if (F == WAVES) {
+            q = blockIdx.x / CG;
             end = tiles_n * row_blocks;
         } else {
-            q = static_cast<int>(min(static_cast<long long>(group) * cut.len, static_cast<long long>(cut.total)));
+            q = static_cast<int>(min(static_cast<long long>(blockIdx.x) * cut.len, static_cast<long long>(cut.total)));
             end = min(q + cut.len, cut.total);
         }
     }
-    __device__ __forceinline__ bool next(LoraSegment &s) {
+    __device__ __forceinline__ bool next(const LoraArgs &g, LoraSegment &s) {
         if (q >= end) return false;
-        if (!WAVES) {
-            s.tile = q / kblocks;
-            s.m0 = 0;
-            s.kb0 = q - s.tile * kblocks;
+        const int rows = g.rows, kblocks = cut.kblocks;
+        if (F != WAVES) {
+            s.unit = q / kblocks;
+            s.tile = F == ONE ? s.unit : s.unit / row_blocks;   // blocks of rows of the same columns behind one another
+            s.m0 = F == ONE ? 0 : (s.unit - s.tile * row_blocks) * rows;
+            s.kb0 = q - s.unit * kblocks;
             s.kb1 = min(kblocks, s.kb0 + end - q);
-            s.part = group - cut.first_cta(s.tile);
-            s.parts = cut.num_parts(s.tile);
+            s.part = static_cast<int>(blockIdx.x) - cut.first_cta(s.unit);
+            s.parts = cut.num_parts(s.unit);
             q += s.kb1 - s.kb0;
-            const int pieces = (m + kChunkRows - 1) / kChunkRows;
+            const int here = F == ONE ? g.M : min(rows, g.M - s.m0), pieces = (here + kChunkRows - 1) / kChunkRows;
             s.own0 = pieces * s.kb0 / kblocks;
             s.own1 = pieces * s.kb1 / kblocks;
+            s.row0 = 0;
+            s.row1 = kChunkRows / 4;
             if (pieces == 1) {
-                const int fours = (m + 3) / 4;
+                const int fours = (here + 3) / 4;
                 s.row0 = fours * s.kb0 / kblocks;
                 s.row1 = fours * s.kb1 / kblocks;
                 s.own0 = 0;
@@ -449,7 +458,7 @@ struct LoraWalker {
             s.kb1 = kblocks;
             s.part = 0;
             s.parts = 1;
-            q += step;
+            q += gridDim.x / CG;
         }
         return true;
     }
@@ -581,36 +590,36 @@ __device__ __forceinline__ bool next_run(const Groups &v, int &at, int &from, in
 
 // Whether the delta warps compute something of piece c for this part of the tile. With few rows the parts of a tile share its pieces, and a
 // single piece by its rows, four at a time: each as many as its share of the K blocks, so that every CTA has the same to do.
-template <bool WAVES>
+template <Form F>
 __device__ __forceinline__ bool has_piece(const LoraSegment &s, const Groups &v, int c) {
-    return WAVES ? (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u : c >= s.own0 && c < s.own1;
+    return F == WAVES ? (v.piece >> (c * kChunkRows / kGroup) & 1u) != 0u : c >= s.own0 && c < s.own1;
 }
 
 // The pieces of one CTA in order: piece c of segment s, rows from s.m0 + c * kChunkRows on.
-template <bool WAVES>
+template <Form F>
 struct PieceWalker {
-    LoraWalker<WAVES> walk;
+    LoraWalker<F> walk;
     LoraSegment s;
     Groups v;
     int c, rows;
-    __device__ __forceinline__ PieceWalker(const LoraWalker<WAVES> &w) : walk(w) { c = rows = 0; }
+    __device__ __forceinline__ PieceWalker(const LoraWalker<F> &w) : walk(w) { c = rows = 0; }
     __device__ __forceinline__ bool next(const LoraArgs &g, int lane) {
         ++c;
         for (;; ++c) {
             while (c * kChunkRows >= rows) {
-                if (!walk.next(s)) return false;
-                if (WAVES) v = tile_groups(g, s.m0, lane);
+                if (!walk.next(g, s)) return false;
+                if (F == WAVES) v = tile_groups(g, s.m0, lane);
                 rows = min(g.rows, g.M - s.m0);
                 c = 0;
             }
-            if (has_piece<WAVES>(s, v, c)) return true;
+            if (has_piece<F>(s, v, c)) return true;
         }
     }
 };
 
-template <typename T, bool WAVES>
+template <typename T, Form F>
 __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __grid_constant__ LoraArgs g) {
-    constexpr int CG = WAVES ? 2 : 1, kSlots = WAVES ? kWaveChunks : kChunks;
+    constexpr int CG = F == WAVES ? 2 : 1, kSlots = F == WAVES ? kWaveChunks : kChunks;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
     constexpr int kBBytes = 128 * 128;                     // 128 rows of B, 64 elements of K
     const uint32_t stage_bytes = kBBytes + g.a_bytes;
     const int stages = g.stages;
-    LoraWalker<WAVES> walk(g);
+    LoraWalker<F> walk(g);
     LoraSegment s;
     int st = 0;
     uint32_t ph = 0;
@@ -665,10 +674,10 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         // -------------------------------------------------------------- operands: TMA
         const bool issuer = elect_one();
         const uint32_t full_leader = CG == 2 ? __shfl_sync(0xffffffffu, mapa_shared(full0, 0), 0) : full0;
-        const uint64_t pol_b = l2_policy(WAVES ? 2 : 1), pol_a = l2_policy(2);
-        for (int n = 0; ok && walk.next(s); ++n) {
+        const uint64_t pol_b = l2_policy(walk.row_blocks > 1 ? 2 : 1), pol_a = l2_policy(2);
+        for (int n = 0; ok && walk.next(g, s); ++n) {
             const int row_b = (s.tile * CG + static_cast<int>(rank)) * 128, row_a = s.m0 + static_cast<int>(rank) * (g.rows / CG);
-            const bool down = WAVES && (n & 1);          // to and fro: the panel ends touched last are still in L2
+            const bool down = F == WAVES && (n & 1);          // to and fro: the panel ends touched last are still in L2
             for (int i = s.kb0; i < s.kb1; ++i) {
                 ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 2000 + st);
                 if (!ok) break;
@@ -686,7 +695,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 }
                 if (++st == stages) st = 0, ph ^= 1u;
             }
-            if constexpr (WAVES) {
+            if constexpr (F == WAVES) {
                 // then the adapters of whole groups: 64 ranks of lora_b and of u's values, the same ranks and u's remainders
                 griddep_wait();
                 const Groups v = tile_groups(g, s.m0, lane);
@@ -711,7 +720,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         // -------------------------------------------------------------- MMA
         if (rank == 0) {
             const bool issuer = elect_one();
-            for (int n = 0; ok && walk.next(s); ++n) {
+            for (int n = 0; ok && walk.next(g, s); ++n) {
                 const int acc = n & 1;
                 ok = wait_warp(acc_empty0 + 8 * acc, ((n >> 1) & 1) ^ 1u, wait, 2100 + acc);
                 if (!ok) break;
@@ -730,7 +739,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                     }
                     if (++st == stages) st = 0, ph ^= 1u;
                 }
-                if constexpr (WAVES) {
+                if constexpr (F == WAVES) {
                     griddep_wait();
                     const Groups v = tile_groups(g, s.m0, lane);
                     int at = 0, from, adapter;
@@ -762,19 +771,19 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         int slot = 0;
         uint32_t slot_ph = 0;
         griddep_wait();                                    // the counters below are zero
-        for (int n = 0; ok && walk.next(s); ++n) {
+        for (int n = 0; ok && walk.next(g, s); ++n) {
             const int acc = n & 1, rows = min(g.rows, g.M - s.m0);
             const int col = (s.tile * CG + static_cast<int>(rank)) * 128 + r;
             const bool mine = col < g.N;
             Groups v_groups = {};
-            if (WAVES) v_groups = tile_groups(g, s.m0, lane);
+            if (F == WAVES) v_groups = tile_groups(g, s.m0, lane);
             ok = wait_warp(acc_full0 + 8 * acc, (n >> 1) & 1, wait, 2300 + acc);
             if (!ok) break;
             tc_fence_after_sync();
             for (int c = 0; c * kChunkRows < rows; ++c) {
                 uint32_t v[16];
                 tmem_ld_32x16(tmem + acc * g.rows + c * kChunkRows + (static_cast<uint32_t>(quarter * 32) << 16), v);
-                const bool add = has_piece<WAVES>(s, v_groups, c);
+                const bool add = has_piece<F>(s, v_groups, c);
                 if (add) ok = wait_warp(delta_full0 + 8 * slot, slot_ph, wait, 2400 + slot);
                 tmem_ld_wait();
                 if (!ok) break;
@@ -809,14 +818,14 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
                 if constexpr (CG == 2) mbar_arrive_cluster(acc_empty_leader + 8 * acc);
                 else mbar_arrive(acc_empty0 + 8 * acc);
             }
-            if (!WAVES && s.parts > 1) {
+            if (F != WAVES && s.parts > 1) {
                 // Four warps of each CTA of the tile's columns count, under the number of the CTA that began them (no CTA begins
                 // two tiles that it does not finish); the CTA whose warp is the last one adds the parts in the end.
                 __threadfence();
                 __syncwarp();
                 if (lane == 0 && atomicAdd(g.arrived + blockIdx.x - s.part, 1) == 4 * s.parts - 1) {
                     __threadfence();
-                    misc[s.kb0 > 0 ? 2 : 3] = s.tile;
+                    misc[s.kb0 > 0 ? 2 : 3] = s.unit;
                 }
             }
         }
@@ -825,7 +834,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         const int w = warp - 6, n = (w & 3) * 32 + lane, half = (w >> 2) * 8;
         int slot = 0, from = 0;
         uint32_t slot_ph = 1, from_ph = 0;
-        PieceWalker<WAVES> at(walk);
+        PieceWalker<F> at(walk);
         griddep_wait();                                    // nothing that this SM's first-level cache may hold is older than the operands
         while (ok && at.next(g, lane)) {
             const int col0 = (at.s.tile * CG + static_cast<int>(rank)) * 128;
@@ -851,7 +860,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         }
     } else {
         // -------------------------------------------------------------- u and the rows' adapters for the warps above
-        PieceWalker<WAVES> at(walk);
+        PieceWalker<F> at(walk);
         int from = 0;
         uint32_t ph_from = 1;
         griddep_wait();                                    // u; and in every CTA: this kernel must not complete before the shrink kernel
@@ -859,7 +868,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
             const int m = at.s.m0 + at.c * kChunkRows + lane;
             const bool there = lane < kChunkRows && m < g.M;
             int id = lane < kChunkRows ? row_adapter(g, m) : kNoRow;
-            if (!WAVES && g.M <= kChunkRows && (lane < 4 * at.s.row0 || lane >= 4 * at.s.row1)) id = -1;
+            if (F != WAVES && (F == BLOCKS || g.M <= kChunkRows) && (lane < 4 * at.s.row0 || lane >= 4 * at.s.row1)) id = -1;
             if (id >= 0) {
                 // what the piece will read of the adapter: 128 of its columns, which lie behind one another
                 const int col = (at.s.tile * CG + static_cast<int>(rank)) * 128;
@@ -884,17 +893,18 @@ __global__ void __launch_bounds__(kLoraThreads, 1) lora_product_kernel(const __g
         cluster_arrive();
         cluster_wait();
     }
-    if (!WAVES && !misc[0]) {
+    if (F != WAVES && !misc[0]) {
         for (int i = 2; i < 4; ++i) {
-            const int tile = misc[i];
-            if (tile < 0) continue;
-            const int parts = walk.cut.num_parts(tile), col = tile * 128 + lane * 4;
+            const int unit = misc[i];
+            if (unit < 0) continue;
+            const int parts = walk.cut.num_parts(unit), tile = F == ONE ? unit : unit / walk.row_blocks, m0 = F == ONE ? 0 : (unit - tile * walk.row_blocks) * g.rows;
+            const int col = tile * 128 + lane * 4, m1 = F == ONE ? g.M : min(m0 + g.rows, g.M);
             if (col >= g.N) continue;
             const int64_t pitch = static_cast<int64_t>(g.M) * g.N;
             constexpr int kWarps = kLoraThreads / 32;
-            for (int m = warp; m < g.M; m += 2 * kWarps) {  // two rows and four parts of each in flight
+            for (int m = m0 + warp; m < m1; m += 2 * kWarps) {  // two rows and four parts of each in flight
                 const float *const o = g.o + static_cast<int64_t>(m) * g.N + col, *const o2 = o + static_cast<int64_t>(kWarps) * g.N;
-                const bool two = m + kWarps < g.M;
+                const bool two = m + kWarps < m1;
                 float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y2 = y;
                 for (int p0 = 0; p0 < parts; p0 += 4) {
                     float4 v[4], v2[4];
@@ -956,8 +966,8 @@ cudaError_t launch_lora(const LoraArgs &g, int smem, cudaStream_t stream) {
         if (e == cudaSuccess) e = launch(lora_join_kernel<T>, g, (g.M + 31) / 32, 32 * (g.rank / 4), 0, 1, stream);
     }
     if (e != cudaSuccess) return e;
-    if (!g.waves) return launch(lora_product_kernel<T, false>, g, g.sms, kLoraThreads, smem, 1, stream);
-    return launch(lora_product_kernel<T, true>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
+    if (!g.waves) return launch(g.rows < g.M ? lora_product_kernel<T, BLOCKS> : lora_product_kernel<T, ONE>, g, g.sms, kLoraThreads, smem, 1, stream);
+    return launch(lora_product_kernel<T, WAVES>, g, g.sms / 2 * 2, kLoraThreads, smem, 2, stream);
 }
 
 // CTAs that may share a tile, one more for stretches that do not start at a tile.
@@ -968,8 +978,8 @@ int most_parts(int64_t units, int64_t kblocks, int64_t groups, int64_t most = kM
 }
 
 struct LoraLayout {
-    bool listed;
-    int parts, parts_u;
+    bool waves, listed;
+    int rows, parts, parts_u;
     int64_t off_u, off_o, off_u16, off_u_parts, off_count, off_adapter, off_entry, off_wide, bytes;
 };
 
@@ -984,20 +994,31 @@ LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int64_t num_adapters, in
     };
     take(kMaxCtas * 4);
     l.off_u = take(M * rank * 4);
-    if (M <= kFewRows) {
+    l.waves = M > kTileRows && (N + 255) / 256 * ((M + 255) / 256) > kLoraGridSms / 8;
+    if (!l.waves) {
+        const int64_t tiles_n = (N + 127) / 128, fewest = (M + kTileRows - 1) / kTileRows, most = (M + 15) / 16;
+        // Blocks of rows: three parts per tile would fill the SMs, or two if a block keeps 96 rows or more, since every block reads B
+        // again (77 x 4104 x 2056 with two blocks: 16.2 -> 20.3 us, 256 x 4096 x 4096, rank 64: 48 -> 41).
+        const int64_t two_parts = kLoraGridSms / 2 / tiles_n, three_parts = kLoraGridSms / 3 / tiles_n;
+        int64_t blocks = M / 96 < two_parts ? M / 96 : two_parts;
+        blocks = blocks < three_parts ? three_parts : blocks;
+        blocks = blocks < fewest ? fewest : blocks > most ? most : blocks;
+        l.rows = static_cast<int>((M + 16 * blocks - 1) / (16 * blocks) * 16);
+        blocks = (M + l.rows - 1) / l.rows;
         // More rows make a part dearer to write and add, the stretches are then kept longer (77 x 4104 x 2056: 16.2 us with
         // four parts, 22.9 with six).
-        l.parts = most_parts((N + 127) / 128, (K + 63) / 64, kLoraGridSms, M > 64 ? 4 : kMaxLoraParts);
+        l.parts = most_parts(tiles_n * blocks, (K + 63) / 64, kLoraGridSms, l.rows > 64 ? 4 : kMaxLoraParts);
         l.off_o = take(l.parts * M * N * 4);
     } else {
+        l.rows = 256;
         l.parts = 2;
         l.off_u16 = take(2 * M * rank * 2);
         l.off_wide = take((M + 31) / 32 * 4);
     }
-    // Up to 256 rows u comes by dot products, which read an adapter for each of its rows, unless that is much more than the products by
+    // Without waves u comes by dot products, which read an adapter for each of its rows, unless that is much more than the products by
     // lists read, which read the rows for each adapter, and enough to pay for two more kernels (256 x 8192 x 8192, rank 64, four
     // adapters: 73 -> 60 us).
-    l.listed = M > kFewRows || (M * rank > 2 * (num_adapters < M ? num_adapters : M) * (256 + rank) && M * rank * K * 2 > (int64_t(64) << 20));
+    l.listed = l.waves || (M * rank > 2 * (num_adapters < M ? num_adapters : M) * (256 + rank) && M * rank * K * 2 > (int64_t(64) << 20));
     if (l.listed) {
         const int64_t blocks = (M + 255) / 256;
         l.parts_u = most_parts(blocks, (K + 63) / 64, kLoraGridSms);
@@ -1022,7 +1043,8 @@ int check_lora(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int rank) 
 
 int prepare_moe_kernels();
 int prepare_routed_kernels() {
-    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, false>, lora_product_kernel<Bf16, true>, lora_product_kernel<Fp16, false>, lora_product_kernel<Fp16, true>};
+    void (*const kernels[])(LoraArgs) = {lora_product_kernel<Bf16, ONE>, lora_product_kernel<Bf16, BLOCKS>, lora_product_kernel<Bf16, WAVES>,
+                                         lora_product_kernel<Fp16, ONE>, lora_product_kernel<Fp16, BLOCKS>, lora_product_kernel<Fp16, WAVES>};
     for (const auto k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return static_cast<int>(e);
@@ -1082,10 +1104,10 @@ extern "C" int b200_gemm_lora(int dtype, const void *A, const void *Bt, void *D,
     g.parts = l.parts;
     g.parts_u = l.parts_u;
     g.listed = l.listed;
-    g.waves = M > kFewRows;
+    g.waves = l.waves;
     const bool bf16 = dtype == B200_BF16;
     const int cg = g.waves ? 2 : 1;
-    g.rows = g.waves ? 256 : static_cast<int>((M + 15) / 16 * 16);
+    g.rows = l.rows;
     const int box_a = g.rows / cg;
     g.wide_b = rank % 16 == 0 && (reinterpret_cast<uintptr_t>(lora_b) & 31u) == 0;
     g.a_bytes = box_a * 128;

@@ -500,6 +500,24 @@ def test_lora_few_adapters_with_many_rows_each(pkg, cuda, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("m, n, k, r, s, order", [(17, 8, 72, 8, 3, "mixed"), (33, 264, 8200, 16, 33, "each"), (90, 520, 1032, 72, 4, "mixed"), (225, 672, 1544, 40, 14, "stretches"),
+                                                  (300, 136, 200, 24, 7, "mixed"), (535, 312, 360, 72, 43, "stretches"), (700, 1160, 264, 128, 5, "mixed"), (1025, 8, 2056, 8, 2, "all"),
+                                                  (2232, 320, 936, 56, 5, "stretches"), (4600, 136, 136, 16, 9, "none")])
+def test_lora_blocks_of_rows(pkg, cuda, name, m, n, k, r, s, order):
+    """Few columns of D: several blocks of rows, each with its own stretch of K blocks; a row's infinite input stays its own."""
+    x, w, a, b, scale = lora_inputs(cuda, name, m, n, k, r, s, m)
+    ids = lora_ids(cuda, order, m, s, m)
+    got = run_lora(pkg, cuda, x, w, a, b, ids, scale)
+    check_close(got, *lora_want(cuda, x, w, a, b, ids, scale), name)
+    x[m // 2, 3] = float("nan")
+    again = run_lora(pkg, cuda, x, w, a, b, ids, scale)
+    assert again[m // 2].isnan().all()
+    rest = cuda.arange(m, device="cuda") != m // 2
+    assert cuda.equal(again[rest], got[rest])
+
+
+@pytest.mark.gpu
 def test_lora_workspace_of_each_number_of_adapters(pkg, cuda):
     """Few adapters need more workspace than many at the same sizes; the calls that allocate it themselves notice."""
     m, n, k, r = 256, 64, 1032, 128
