@@ -1017,8 +1017,9 @@ LoraLayout lora_layout(int64_t M, int64_t N, int64_t K, int64_t num_adapters, in
     }
     // Without waves u comes by dot products, which read an adapter for each of its rows, unless that is much more than the products by
     // lists read, which read the rows for each adapter, and enough to pay for two more kernels (256 x 8192 x 8192, rank 64, four
-    // adapters: 73 -> 60 us).
-    l.listed = l.waves || (M * rank > 2 * (num_adapters < M ? num_adapters : M) * (256 + rank) && M * rank * K * 2 > (int64_t(64) << 20));
+    // adapters: 73 -> 60 us). Beyond 256 rows requests bring many rows each, however many adapters there are to choose from.
+    const bool few_adapters = M > kTileRows || M * rank > 2 * (num_adapters < M ? num_adapters : M) * (256 + rank);
+    l.listed = l.waves || (few_adapters && M * rank * K * 2 > (int64_t(64) << 20));
     if (l.listed) {
         const int64_t blocks = (M + 255) / 256;
         l.parts_u = most_parts(blocks, (K + 63) / 64, kLoraGridSms);

@@ -503,7 +503,7 @@ def test_lora_few_adapters_with_many_rows_each(pkg, cuda, m):
 @pytest.mark.parametrize("name", ["bf16", "fp16"])
 @pytest.mark.parametrize("m, n, k, r, s, order", [(17, 8, 72, 8, 3, "mixed"), (33, 264, 8200, 16, 33, "each"), (90, 520, 1032, 72, 4, "mixed"), (225, 672, 1544, 40, 14, "stretches"),
                                                   (300, 136, 200, 24, 7, "mixed"), (535, 312, 360, 72, 43, "stretches"), (700, 1160, 264, 128, 5, "mixed"), (1025, 8, 2056, 8, 2, "all"),
-                                                  (2232, 320, 936, 56, 5, "stretches"), (4600, 136, 136, 16, 9, "none")])
+                                                  (2232, 320, 936, 56, 5, "stretches"), (1100, 264, 1032, 32, 200, "stretches"), (4600, 136, 136, 16, 9, "none")])
 def test_lora_blocks_of_rows(pkg, cuda, name, m, n, k, r, s, order):
     """Few columns of D: several blocks of rows, each with its own stretch of K blocks; a row's infinite input stays its own."""
     x, w, a, b, scale = lora_inputs(cuda, name, m, n, k, r, s, m)
