@@ -10,19 +10,23 @@
 // that many partial sums ("parts") in the workspace, which the next kernel adds in ascending order: no CTA waits for
 // another, nothing is accumulated atomically, the same inputs give the same bits.
 //
-// Up to 128 (token, choice) pairs, two kernels:
+// Up to 128 (token, choice) pairs, two kernels (three with fp16):
 //   moe_product_kernel<UP_FEW>    every CTA makes the router's choice for itself (the logits are few), then its stretch of G and U: a tile
 //                                 is 64 rows of G and the same 64 rows of U; sums (fp32) to the workspace
 //   moe_product_kernel<DOWN_FEW>  a tile is 128 rows of W2; loader warps add the parts of a K block, apply silu and the gate, and hand the
 //                                 result to the tensor core as a pair of 16-bit numbers, value and remainder (two MMAs per
 //                                 K step: the tensor core idles here, and one 16-bit rounding of the gated value would
 //                                 cost as much accuracy as the rounding of the result); the last CTA of a tile of Y adds
-//                                 its parts and the weighted choices
+//                                 its parts and the weighted choices. With fp16 the pairs have to be scaled, for which a
+//                                 slot's largest value has to be known: moe_gate_kernel makes them in between, at the price of
+//                                 a kernel in the chain (2 tokens, 8 experts of 1024 x 512, top 2: 15.6 us with bf16, 20.0 with
+//                                 fp16; one token, 8 of 128 experts of 2048 x 768: 28.5 and 33; 16 tokens, 64 experts of 4096 x
+//                                 2048, top 6: 398 and 405)
 // beyond that five, because each CTA would spend too long on the choice, the gated values and the last sums (48 tokens, 32 experts
 // of 1024 x 512, top 4: 38 against 41 us; 256 tokens, 128 experts of 2048 x 768, top 8: 230 against 404):
 //   moe_route_kernel              a cluster of up to eight blocks: the choice per token (one warp each), the chosen experts' tokens
 //   moe_product_kernel<UP>        as above, with two 64 + 64 row atoms per tile
-//   moe_gate_kernel               the gated values of all slots, as pairs
+//   moe_gate_kernel               the gated values of all slots, as pairs, scaled with fp16
 //   moe_product_kernel<DOWN>      as above, the pairs by TMA, two 128-row atoms per tile
 //   moe_combine_kernel            parts and weighted choices of a token, one rounding
 //
@@ -53,12 +57,15 @@ constexpr int kTileWords = kMaxHidden / 128 / 32;   // a bit per tile of Y
 constexpr int kFewSlots = 128;      // (token, choice) pairs and tokens up to which two kernels do all of it; the tokens also
 constexpr int kFewTokens = 64;      // bound a stage of the smaller ring, which must hold two
 constexpr int kGridSms = 148;       // what the workspace is sized for; another count only changes how tiles are cut
+constexpr int kGateThreads = 256;   // most threads of a block of moe_gate_kernel, most blocks of a slot, quads that a thread keeps
+constexpr int kGateBlocks = 8;
+constexpr int kGateQuads = 2;
 constexpr int kBoxBytes = 16 * 128;      // 16 slots of 64 gated values
 constexpr int kWeightBytes = 128 * 128;  // one K block of a weight tile: 128 rows of 64 elements
 
 // What the route kernel leaves for the others, in the workspace.
 struct Lists {
-    int *header;     // [0] chosen experts, [1] most tokens of one
+    int *header;     // [0] chosen experts, [1] most tokens of one, [2] slots
     int *expert;     // per chosen expert: its index, its number of tokens, the first of its slots
     int *count;
     int *base;
@@ -67,6 +74,7 @@ struct Lists {
     int *slot;       // per (token, choice): its slot, -1 without one
     int *active;     // per (token, choice): the position of its expert in the list of chosen ones
     float *weight;   // per (token, choice)
+    float *unscale;  // per slot, fp16: the power of two that its gated values, as DOWN sees them, have to be multiplied with
 };
 
 struct alignas(64) MoeArgs {
@@ -80,7 +88,7 @@ struct alignas(64) MoeArgs {
     Lists list;
     float *z;                 // [part][slot][2 * inner]: sums of UP
     float *o;                 // [part][slot][hidden]: sums of DOWN
-    uint16_t *h;              // [value, remainder][slot][inner]: gated values
+    uint16_t *h;              // [value, remainder][slot][inner]: gated values, scaled
     int tokens, hidden, inner, experts, top_k, normalise, slots;
     int parts_up, parts_down;
     int sms;
@@ -168,9 +176,9 @@ __device__ __forceinline__ void choose(const MoeArgs &g, int t, int lane, int &i
 }
 
 // One warp: emit(position among the chosen, expert, tokens, first slot) for every expert that a token chose, in ascending order;
-// mask[e * words ..] holds the tokens of expert e as bits. Returns how many are chosen and the most tokens of one.
+// mask[e * words ..] holds the tokens of expert e as bits. Returns how many are chosen, the most tokens of one, and the slots.
 template <typename Emit>
-__device__ __forceinline__ int2 list_experts(const uint32_t *mask, int words, int experts, int lane, Emit emit) {
+__device__ __forceinline__ int3 list_experts(const uint32_t *mask, int words, int experts, int lane, Emit emit) {
     int chosen = 0, slots = 0, most = 0;
     for (int e0 = 0; e0 < experts; e0 += 32) {
         const int e = e0 + lane;
@@ -190,7 +198,7 @@ __device__ __forceinline__ int2 list_experts(const uint32_t *mask, int words, in
         slots += __shfl_sync(0xffffffffu, before, 31);
         most = max(most, static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(n))));
     }
-    return make_int2(chosen, most);
+    return make_int3(chosen, most, slots);
 }
 
 // The place of token t among the tokens of its expert.
@@ -229,7 +237,7 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__
     cluster_wait();
     if (blockIdx.x != 0) return;
     if (warp == 0) {
-        const int2 n = list_experts(mask, words, g.experts, lane, [&](int at, int e, int count, int base) {
+        const int3 n = list_experts(mask, words, g.experts, lane, [&](int at, int e, int count, int base) {
             g.list.expert[at] = e;
             g.list.count[at] = count;
             g.list.base[at] = base;
@@ -239,6 +247,7 @@ __global__ void __launch_bounds__(1024) moe_route_kernel(const __grid_constant__
         if (lane == 0) {
             g.list.header[0] = n.x;
             g.list.header[1] = n.y;
+            g.list.header[2] = n.z;
         }
     }
     __syncthreads();
@@ -298,11 +307,10 @@ enum Product {
                // of Y adds the tile's parts
 };
 
-// The gated value of four neighbouring inner rows of one slot from UP's parts (ascending, BATCH of them in flight), as pairs of
-// 16-bit numbers. The exponential and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th
-// of an fp16.
-template <typename T, int BATCH>
-__device__ __forceinline__ void gated_values(const float *z, int inner, int parts, int64_t part_pitch, uint2 &hi, uint2 &lo) {
+// The gated values of four neighbouring inner rows of one slot from UP's parts (ascending, BATCH of them in flight). The exponential
+// and the quotient err by 2^-21 together: a 128th of what the pair keeps of a bf16, an 8th of an fp16.
+template <int BATCH>
+__device__ __forceinline__ float4 gated_values(const float *z, int inner, int parts, int64_t part_pitch) {
     float4 gate = make_float4(0.0f, 0.0f, 0.0f, 0.0f), up = gate;
     for (int p0 = 0; p0 < parts; p0 += BATCH, z += BATCH * part_pitch) {
         float4 a[BATCH], b[BATCH];
@@ -319,10 +327,17 @@ __device__ __forceinline__ void gated_values(const float *z, int inner, int part
                 up.x += b[p].x, up.y += b[p].y, up.z += b[p].z, up.w += b[p].w;
             }
     }
-    const float g[4] = {gate.x, gate.y, gate.z, gate.w}, u[4] = {up.x, up.y, up.z, up.w};
+    const auto gated = [](float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; };
+    return make_float4(gated(gate.x, up.x), gated(gate.y, up.y), gated(gate.z, up.z), gated(gate.w, up.w));
+}
+
+template <typename T>
+__device__ __forceinline__ void split_four(const float4 &v, uint2 &hi, uint2 &lo) {   // as pairs of 16-bit numbers
     uint16_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) T::split(__fdividef(g[i], 1.0f + __expf(-g[i])) * u[i], h[i], l[i]);
+    T::split(v.x, h[0], l[0]);
+    T::split(v.y, h[1], l[1]);
+    T::split(v.z, h[2], l[2]);
+    T::split(v.w, h[3], l[3]);
     hi = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
     lo = make_uint2(l[0] | static_cast<uint32_t>(l[1]) << 16, l[2] | static_cast<uint32_t>(l[3]) << 16);
 }
@@ -365,6 +380,7 @@ __device__ __forceinline__ void combine(const MoeArgs &g, int2 *entry, int t, in
 template <typename T, Product P>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __grid_constant__ MoeArgs g) {
     constexpr bool kUp = P == UP || P == UP_FEW, kFew = P == UP_FEW || P == DOWN_FEW;
+    constexpr bool kGated = P == DOWN || (P == DOWN_FEW && T::kScaled);   // moe_gate_kernel has left the gated values
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -386,7 +402,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
 
     if (tid < 2 * kMoeStages + 4) {
         // full: the producer's byte count and four arrivals of the loader warps; accumulator empty: the four draining warps
-        mbar_init(full0 + 8 * tid, tid < kMoeStages ? (P == DOWN ? 1 : 5) : tid < 2 * kMoeStages + 2 ? 1 : 4);
+        mbar_init(full0 + 8 * tid, tid < kMoeStages ? (kGated ? 1 : 5) : tid < 2 * kMoeStages + 2 ? 1 : 4);
         fence_mbar_init();
     }
     if (tid == 0) misc[0] = 0;
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     if (kFew)
         for (int i = tid; i < g.experts * words; i += kMoeThreads) mask_s[i] = 0u;
     if (tid == 32) tma_prefetch_desc(&g.map);
-    if (P == DOWN && tid == 64) tma_prefetch_desc(&g.map_h);
+    if (kGated && tid == 64) tma_prefetch_desc(&g.map_h);
     if (warp == 1) {
         tmem_alloc<1>(ring + g.off_misc + 4, g.tmem_cols);
         tmem_relinquish<1>();
@@ -427,6 +443,10 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                 if (kUp && blockIdx.x == 0) {
                     if (g.ids_out) g.ids_out[lane] = id;
                     if (g.weights_out) g.weights_out[lane] = w;
+                    if (T::kScaled) {
+                        g.list.owner[lane] = lane;
+                        if (lane == 0) g.list.header[0] = g.list.header[2] = n;
+                    }
                 }
             }
             if (lane == 0) misc[2] = n, misc[3] = n > 0;
@@ -449,13 +469,16 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         }
         __syncthreads();
         if (warp == 0) {
-            const int2 n = list_experts(mask_s, words, g.experts, lane, [&](int at, int e, int count, int base) {
+            const int3 n = list_experts(mask_s, words, g.experts, lane, [&](int at, int e, int count, int base) {
                 expert_s[at] = e;
                 count_s[at] = count;
                 base_s[at] = base;
                 place_s[e] = static_cast<int16_t>(at);
             });
-            if (lane == 0) misc[2] = n.x, misc[3] = n.y;
+            if (lane == 0) {
+                misc[2] = n.x, misc[3] = n.y;
+                if (kUp && T::kScaled && blockIdx.x == 0) g.list.header[0] = n.x, g.list.header[2] = n.z;
+            }
         }
         __syncthreads();
         for (int at = tid; at < g.slots; at += kMoeThreads) {
@@ -465,6 +488,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
             token_s[slot] = static_cast<uint16_t>(t);
             slot_s[at] = static_cast<int16_t>(slot);
             active_s[at] = place_s[e];
+            if (kUp && T::kScaled && blockIdx.x == 0) g.list.owner[slot] = place_s[e];
         }
     } else {
         const int n = __ldcg(g.list.header);
@@ -502,7 +526,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         Walker<P == DOWN_FEW> ahead = walk;
         Segment f;
         int fst = 0, fkb = 0, filled = 0;
-        if (P == DOWN) {
+        if (kGated) {
             // the weights of the first stages do not depend on the kernels before: on their way before the wait
             while (filled < stages && ahead.next(f)) {
                 const int row = expert_s[f.ai] * g.hidden + f.tile * atoms * 128, na = min(atoms, blocks - f.tile * atoms);
@@ -520,14 +544,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
             const int row = kUp ? e * 2 * g.inner + s.tile * atoms * 64 : e * g.hidden + s.tile * atoms * 128;
             const int na = min(atoms, blocks - s.tile * atoms);
             for (int kb = s.kb0; kb < s.kb1; ++kb) {
-                if (P == DOWN && filled > 0) {
+                if (kGated && filled > 0) {
                     --filled;                              // its weights are on their way
                 } else {
                     ok = wait_warp(empty0 + 8 * st, ph ^ 1u, wait, 1000 + st);
                     if (!ok) break;
                     if (issuer) {
                         const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes;
-                        mbar_arrive_expect_tx(bar, kWeightBytes * na + (P == DOWN ? boxes * 2 * kBoxBytes : 0));
+                        mbar_arrive_expect_tx(bar, kWeightBytes * na + (kGated ? boxes * 2 * kBoxBytes : 0));
                         for (int a = 0; a < na; ++a) {
                             const uint32_t to = dst + a * kWeightBytes;
                             tma_load_2d_hint(to, &g.map, bar, kb * 64, row + a * (kUp ? 64 : 128), once);
@@ -535,7 +559,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                         }
                     }
                 }
-                if (P == DOWN && issuer) {
+                if (kGated && issuer) {
                     const uint32_t bar = full0 + 8 * st, dst = ring + st * stage_bytes + rows_at;
                     for (int b = 0; b < boxes; ++b) {
                         tma_load_2d(dst + b * kBoxBytes, &g.map_h, bar, kb * 64, base_s[s.ai] + 16 * b);
@@ -639,7 +663,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
         }
         if (P == DOWN_FEW && chosen == 0)
             for (int i = blockIdx.x * 128 + r; i < g.tokens * g.hidden; i += gridDim.x * 128) g.Y[i] = 0;
-    } else if (P != DOWN) {
+    } else if (!kGated) {
         // -------------------------------------------------------------- activations
         // The loader warps form groups that take the K blocks in turn, so that the latency of a block's loads is spread over
         // several blocks. A group looks at a stage only when its own turn comes; the phase it waits for cannot be
@@ -672,7 +696,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                         const int parts = up.num_parts(s.ai * tiles_up + kb), k4 = kb * 64 + (lane & 15) * 4;
                         for (int r = row0; r < count; r += row_step) {
                             uint2 hi = make_uint2(0, 0), lo = hi;
-                            if (k4 < g.inner) gated_values<T, 4>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k4, g.inner, parts, part_pitch, hi, lo);
+                            if (k4 < g.inner) split_four<T>(gated_values<4>(g.z + static_cast<int64_t>(base + r) * 2 * g.inner + k4, g.inner, parts, part_pitch), hi, lo);
                             const uint32_t at = dst + swizzled(r, (lane & 15) >> 1) + (lane & 1) * 8;
                             st_shared_v2(at, hi);
                             st_shared_v2(at + rows_bytes, lo);
@@ -702,6 +726,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
                     slot = slot_s[t * g.top_k + lane];
                     w = weight_s[t * g.top_k + lane];
                     if (slot >= 0) parts = cut.num_parts(tile * chosen + active_s[t * g.top_k + lane]);
+                    if (T::kScaled && slot >= 0) w *= __ldcg(g.list.unscale + slot);
                 }
                 combine<T>(g, entry, t, tile * 128 + lane * 4, lane, slot, parts, w);
             }
@@ -718,25 +743,74 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_product_kernel(const __gri
     }
 }
 
-// The gated values for DOWN: four inner rows of one slot per thread. Where it has much to do a slot's values come in one or two parts, so
-// more threads per SM serve better than more parts in flight (256 tokens, 128 experts of 2048 x 768, top 8: 232 us for
-// the layer with four, 228 with two; 129 tokens, 7 experts of 1560 x 248, many parts: 37 against 38).
-template <typename T>
-__global__ void __launch_bounds__(256) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
+// The gated values for DOWN, up to eight blocks per slot. A pair of fp16 numbers keeps an absolute 2^-25 and holds nothing beyond 2 *
+// 65504, so with fp16 the blocks of a slot, a cluster, first find its largest finite value and scale by the power of two that
+// brings it to 2^14 .. 2^15: each value then errs by 2^-22 of itself and 2^-39 of the largest. The sums of DOWN, which are kept
+// per slot, are multiplied back exactly with the choice's weight (factors beyond 2^100 would leave the range of fp32 there).
+// A pair of bf16 numbers keeps 2^-16 of any value as it is.
+// A slot's values come in one or two parts where there is much to do, so more threads per SM serve better than more parts in
+// flight (256 tokens, 128 experts of 2048 x 768, top 8: 232 us for the layer with four, 228 with two). What a thread computes
+// for the maximum it keeps, as long as that is kGateQuads quads.
+template <typename T, bool FEW>
+__global__ void __launch_bounds__(kGateThreads, 4) moe_gate_kernel(const __grid_constant__ MoeArgs g) {
+    __shared__ uint32_t largest_s[kGateBlocks * kGateThreads / 32];
+    const bool cluster = T::kScaled && gridDim.x > 1;
     griddep_launch_dependents();   // DOWN reads nothing of this kernel before its own wait
+    if (cluster) cluster_arrive();
     griddep_wait();
-    const int slot = blockIdx.y, k = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-    const int chosen = __ldcg(g.list.header), most = __ldcg(g.list.header + 1), owner = __ldcg(g.list.owner + slot);
-    if (k >= g.inner || chosen == 0) return;
-    // slots behind the last one are nobody's: their entries are what the workspace held
-    if (slot >= __ldcg(g.list.base + chosen - 1) + __ldcg(g.list.count + chosen - 1)) return;
-    const int atoms = tile_atoms(g, most), tiles = ((g.inner + 63) / 64 + atoms - 1) / atoms;
+    if (cluster) cluster_wait();   // every block runs: its shared memory may be written
+    const int slot = blockIdx.y, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int chosen = __ldcg(g.list.header), most = FEW ? 0 : __ldcg(g.list.header + 1), slots = __ldcg(g.list.header + 2), owner = __ldcg(g.list.owner + slot);
+    if (slot >= slots) return;     // nobody's: its entries are what the workspace held
+    const int atoms = FEW ? 1 : tile_atoms(g, most), tiles = ((g.inner + 63) / 64 + atoms - 1) / atoms;
     const Cut up(chosen * tiles, (g.hidden + 63) / 64, g.sms, g.parts_up);
-    uint2 hi, lo;
-    gated_values<T, 2>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(owner * tiles + k / 64 / atoms),
-                    static_cast<int64_t>(g.slots) * 2 * g.inner, hi, lo);
-    *reinterpret_cast<uint2 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = hi;
-    *reinterpret_cast<uint2 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = lo;
+    const auto values = [&](int k) {
+        return gated_values<2>(g.z + static_cast<int64_t>(slot) * 2 * g.inner + k, g.inner, up.num_parts(owner * tiles + k / 64 / atoms),
+                               static_cast<int64_t>(g.slots) * 2 * g.inner);
+    };
+    const int first = (blockIdx.x * blockDim.x + threadIdx.x) * 4, step = gridDim.x * blockDim.x * 4, span = step * kGateQuads;
+    float4 v[kGateQuads];
+    float scale = 1.0f;
+    if constexpr (T::kScaled) {
+        const auto size = [](float f) {   // of a finite number, as bits that compare like it
+            const uint32_t b = __float_as_uint(f) & 0x7fffffffu;
+            return b < 0x7f800000u ? b : 0u;
+        };
+        uint32_t largest = 0u;
+        for (int k0 = first; k0 < g.inner; k0 += span)
+#pragma unroll
+            for (int i = 0; i < kGateQuads; ++i)
+                if (k0 + i * step < g.inner) {
+                    v[i] = values(k0 + i * step);
+                    largest = max(max(max(largest, size(v[i].x)), max(size(v[i].y), size(v[i].z))), size(v[i].w));
+                }
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        if (cluster) {   // every warp tells every block
+            if (lane < gridDim.x) st_cluster(mapa_shared(smem_u32(&largest_s[blockIdx.x * warps + (threadIdx.x >> 5)]), lane), largest);
+            cluster_arrive();
+            cluster_wait();
+        } else {
+            if (lane == 0) largest_s[threadIdx.x >> 5] = largest;
+            __syncthreads();
+        }
+        largest = 0u;
+        for (int w = lane; w < gridDim.x * warps; w += 32) largest = max(largest, largest_s[w]);
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        const int shift = min(max(127 + 14 - static_cast<int>(largest >> 23), -100), 100);
+        scale = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+        if (blockIdx.x == 0 && threadIdx.x == 0) g.list.unscale[slot] = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+    }
+    for (int k0 = first; k0 < g.inner; k0 += span)
+#pragma unroll
+        for (int i = 0; i < kGateQuads; ++i) {
+            const int k = k0 + i * step;
+            if (k >= g.inner) continue;
+            if (!T::kScaled || g.inner > span) v[i] = values(k);
+            uint2 hi, lo;
+            split_four<T>(make_float4(v[i].x * scale, v[i].y * scale, v[i].z * scale, v[i].w * scale), hi, lo);
+            *reinterpret_cast<uint2 *>(g.h + static_cast<int64_t>(slot) * g.inner + k) = hi;
+            *reinterpret_cast<uint2 *>(g.h + (static_cast<int64_t>(g.slots) + slot) * g.inner + k) = lo;
+        }
 }
 
 template <typename T>
@@ -754,6 +828,7 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant_
         const int at = t * g.top_k + lane;
         slot = __ldcg(g.list.slot + at);
         w = __ldcg(g.list.weight + at);
+        if (T::kScaled && slot >= 0) w *= __ldcg(g.list.unscale + slot);
         if (slot >= 0 && block < blocks) parts = cut.num_parts(__ldcg(g.list.active + at) * tiles + block / atoms);
     }
     combine<T>(g, entry[warp], t, block * 128 + lane * 4, lane, slot, parts, w);
@@ -779,7 +854,7 @@ int most_parts(int64_t units, int64_t kblocks) {
 struct MoeLayout {
     int parts_up, parts_down;
     bool few;
-    int64_t off_list, off_z, off_o, off_h, bytes;   // few: the list is the counters of the tiles
+    int64_t off_list, off_z, off_o, off_h, bytes;   // few: the counters of the tiles before the list
 };
 
 MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int top_k) {
@@ -787,12 +862,12 @@ MoeLayout moe_layout(int64_t tokens, int64_t hidden, int64_t inner, int64_t expe
     const int64_t slots = tokens * top_k, up_tiles = (inner + 63) / 64;
     l.parts_up = most_parts(top_k * up_tiles, (hidden + 63) / 64);
     l.parts_down = most_parts(top_k * ((hidden + 127) / 128), up_tiles);
-    l.off_list = 0;
     l.few = slots <= kFewSlots && tokens <= kFewTokens;
-    l.off_z = l.few ? up256((hidden + 127) / 128 * 4) : up256((2 + 3 * experts + 5 * slots) * 4);
+    l.off_list = l.few ? up256((hidden + 127) / 128 * 4) : 0;
+    l.off_z = l.off_list + up256((3 + 3 * experts + 6 * slots) * 4);
     l.off_o = l.off_z + up256(l.parts_up * slots * 2 * inner * 4);
     l.off_h = l.off_o + up256(l.parts_down * slots * hidden * 4);
-    l.bytes = l.off_h + (l.few ? 0 : up256(2 * slots * inner * 2));
+    l.bytes = l.off_h + up256(2 * slots * inner * 2);
     return l;
 }
 
@@ -814,20 +889,31 @@ cudaError_t launch(Kernel *kernel, const MoeArgs &g, dim3 grid, int threads, int
     return cudaLaunchKernelEx(&cfg, kernel, g);
 }
 
+template <typename Kernel>
+cudaError_t launch_gate(Kernel *kernel, const MoeArgs &g, cudaStream_t stream) {
+    const int quads = g.inner / 4, threads = quads >= kGateThreads ? kGateThreads : (quads + 31) / 32 * 32;
+    int blocks = 1;
+    while (blocks < kGateBlocks && blocks * threads * kGateQuads < quads) blocks *= 2;
+    return launch(kernel, g, dim3(blocks, g.slots), threads, 0, blocks, stream);
+}
+
 template <typename T>
 cudaError_t launch_moe(MoeArgs &g, const CUtensorMap &up, const CUtensorMap &down, bool few, int smem, cudaStream_t stream) {
     g.map = up;
     if (few) {
         const cudaError_t e = launch(moe_product_kernel<T, UP_FEW>, g, g.sms, kMoeThreads, smem, 0, stream);
         if (e != cudaSuccess) return e;
+        if constexpr (T::kScaled) {
+            const cudaError_t gate = launch_gate(moe_gate_kernel<T, true>, g, stream);
+            if (gate != cudaSuccess) return gate;
+        }
         g.map = down;
         return launch(moe_product_kernel<T, DOWN_FEW>, g, g.sms, kMoeThreads, smem, 0, stream);
     }
     const int blocks = (g.tokens + 31) / 32;
     cudaError_t e = launch(moe_route_kernel, g, blocks, 1024, 0, blocks, stream);
     if (e == cudaSuccess) e = launch(moe_product_kernel<T, UP>, g, g.sms, kMoeThreads, smem, 0, stream);
-    const int quads = g.inner / 4, threads = quads >= 256 ? 256 : (quads + 31) / 32 * 32;
-    if (e == cudaSuccess) e = launch(moe_gate_kernel<T>, g, dim3((quads + threads - 1) / threads, g.slots), threads, 0, 0, stream);
+    if (e == cudaSuccess) e = launch_gate(moe_gate_kernel<T, false>, g, stream);
     g.map = down;
     if (e == cudaSuccess) e = launch(moe_product_kernel<T, DOWN>, g, g.sms, kMoeThreads, smem, 0, stream);
     if (e == cudaSuccess) e = launch(moe_combine_kernel<T>, g, dim3((g.hidden + 511) / 512, g.tokens), 128, 0, 0, stream);
@@ -885,12 +971,12 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     const int64_t slots = tokens * top_k;
     g.h = reinterpret_cast<uint16_t *>(ws + l.off_h);
-    if (st == B200_OK && !l.few) st = encode_operand_map(&g.map_h, dtype, g.h, inner, 2 * slots, 16);
+    if (st == B200_OK && (!l.few || dtype == B200_F16)) st = encode_operand_map(&g.map_h, dtype, g.h, inner, 2 * slots, 16);
     if (st != B200_OK) return st;
     int *const list = reinterpret_cast<int *>(ws + l.off_list);
-    g.arrived = list;
+    g.arrived = reinterpret_cast<int *>(ws);
     g.list.header = list;
-    g.list.expert = list + 2;
+    g.list.expert = list + 3;
     g.list.count = g.list.expert + experts;
     g.list.base = g.list.count + experts;
     g.list.token = g.list.base + experts;
@@ -898,6 +984,7 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     g.list.slot = g.list.owner + slots;
     g.list.active = g.list.slot + slots;
     g.list.weight = reinterpret_cast<float *>(g.list.active + slots);
+    g.list.unscale = g.list.weight + slots;
     g.z = reinterpret_cast<float *>(ws + l.off_z);
     g.o = reinterpret_cast<float *>(ws + l.off_o);
     g.X = static_cast<const uint16_t *>(X);
@@ -921,7 +1008,9 @@ extern "C" int b200_moe(int dtype, const void *X, const float *logits, const voi
     if (g.tmem_cols > kTmemColumns) g.tmem_cols = kTmemColumns;
     const int slot_lists = static_cast<int>(up256(slots * (l.few ? 10 : 2)));
     const int expert_lists = static_cast<int>(up256(experts * (12 + (l.few ? (tokens + 31) / 32 * 4 + 2 : 0))));
-    const int smem = l.few ? 113 * 1024 : kSmemLimit;   // two blocks of 114 KB each are an SM's 228
+    // Two blocks and the KB that the hardware takes for each fit an SM's 228; with fp16 a block of the gate kernel fits beside them (37 tokens,
+    // 20 experts of 1000 x 360, top 3: 31.0 us, 32.5 where it does not).
+    const int smem = l.few ? (dtype == B200_F16 ? 112 : 113) * 1024 : kSmemLimit;
     g.ring_bytes = (smem - 1024 - slot_lists - expert_lists - 512) / 1024 * 1024;
     g.off_slots = g.ring_bytes;
     g.off_experts = g.off_slots + slot_lists;

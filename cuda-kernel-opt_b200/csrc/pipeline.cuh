@@ -53,6 +53,11 @@ __device__ __forceinline__ void red_or_cluster(uint32_t cluster_addr, uint32_t b
     asm volatile("red.shared::cluster.or.b32 [%0], %1;" ::"r"(cluster_addr), "r"(bits) : "memory");
 }
 
+// A word of another CTA's shared memory (address from mapa_shared).
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
 // Completes `bar` when the MMAs issued before have; for a pair (the two CTAs of a cluster) the barrier at this place in both.
 template <int CG>
 __device__ __forceinline__ void commit_cta(uint32_t bar) {
