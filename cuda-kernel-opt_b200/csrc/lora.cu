@@ -10,7 +10,7 @@
 // Why not on the tensor core, as further columns of K: the zero that stands for "not this row's adapter" does not mask an infinity
 // or a NaN among an adapter's weights, so a request would see other requests' adapters; and a decode step in which every
 // row has another adapter would feed it one useful row at a time. Only where 32 rows in a row have one adapter, as in a
-// prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder).
+// prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder), as long as u fits those.
 //
 // Three forms, by the numbers of rows and columns:
 //   up to 256     one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s; 128
@@ -70,7 +70,7 @@ struct alignas(64) LoraArgs {
     uint16_t *u16;                 // [value, remainder][M][rank]
     struct {
         int *count, *adapter, *entry;   // per block of 256 rows: adapters that occur, and which; per row: which of them it has
-        int *wide;                 // per 32 rows: some u does not fit a pair of 16-bit numbers
+        int *wide;                 // per 32 rows: u does not fit pairs of 16-bit numbers
     } list;
     int waves;                     // the form of the product: its own parameter, the last pass of many rows may be short
     int listed, parts_u, on_tensor;   // u by lists of adapters; its parts; whether the adapters' second product may use the tensor core
@@ -357,7 +357,11 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_kernel(const __
 }
 
 // u from its parts, ascending: 32 rows per block, four ranks of one row per thread; as floats and as pairs of 16-bit numbers, and whether the
-// rows' u fit those.
+// rows' u fit those: no value beyond the type's range, and the largest of eight neighbouring ranks not so small that the pair's
+// absolute error, half of the smallest step (fp16: 2^-25), is more than 2^-17 of it. Judging each value by itself would keep ordinary
+// rows off the tensor core, in which some of the values are always small; judging whole rows would let adapters that are
+// stacked along the rank hide one another. (4096 x 8192 x 8192, eight prompts, fp16, u of ordinary size against u of 10^-5: rank
+// 64 some 410 and 650 us, rank 128 some 430 and 880.)
 template <typename T>
 __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__ LoraArgs g) {
     __shared__ int before[kMaxBlocks + 1];
@@ -370,6 +374,7 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
     if (threadIdx.x < 32) scan_lists(g, blocks, threadIdx.x, before);
     __syncthreads();
     bool fits = true;
+    float largest = 0.0f;
     if (entry >= 0) {
         const Cut cut(before[blocks], (g.K + 63) / 64, g.sms, g.parts_u);
         const int parts = cut.num_parts(before[m >> 8] + entry);
@@ -389,6 +394,7 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
             f[j] *= scale;
             T::split(f[j], hi[j], lo[j]);
             fits = fits && fabsf(f[j]) <= T::kMax;
+            largest = fmaxf(largest, fabsf(f[j]));
         }
         *reinterpret_cast<float4 *>(g.u + static_cast<int64_t>(m) * g.rank + r) = make_float4(f[0], f[1], f[2], f[3]);
         if (g.waves) {
@@ -396,6 +402,8 @@ __global__ void __launch_bounds__(1024) lora_join_kernel(const __grid_constant__
             *reinterpret_cast<uint2 *>(g.u16 + (static_cast<int64_t>(g.M) + m) * g.rank + r) = make_uint2(lo[0] | static_cast<uint32_t>(lo[1]) << 16, lo[2] | static_cast<uint32_t>(lo[3]) << 16);
         }
     }
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));   // the neighbour has the same row: a row's threads are an even number
+    fits = fits && (largest == 0.0f || largest >= T::kPairMin);
     const int all = __syncthreads_and(fits);
     if (g.waves && threadIdx.x == 0) g.list.wide[blockIdx.x] = !all;
 }

@@ -15,6 +15,7 @@ struct Bf16 {
     static constexpr int kCode = B200_BF16;
     static constexpr float kMax = 3.38953139e38f;
     static constexpr bool kScaled = false;   // whether a pair (see split) loses what a float holds unless it is scaled
+    static constexpr float kPairMin = 0x1p-100f;   // from here on a pair errs by 2^-16 at most, and what is smaller by 2^-17 of this
     // two packed elements -> two floats; element 0 sits in the low half
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -32,6 +33,7 @@ struct Fp16 {
     static constexpr int kCode = B200_F16;
     static constexpr float kMax = 65504.0f;
     static constexpr bool kScaled = true;
+    static constexpr float kPairMin = 0x1p-8f;     // 2^-25 / 2^-17
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return __half22float2(*reinterpret_cast<const __half2 *>(&v));
     }
