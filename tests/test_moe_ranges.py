@@ -4,11 +4,13 @@ pairs of 16-bit numbers, and fp16 has neither numbers beyond 65504 nor steps bel
 The layers of `one_number_each` make every element of Y a single gated value times a power of two, with a gate and an up
 product that are exact in fp32, so that what the layer does to the gated value can be bounded tightly:
 
-    exponential      2 units in the last place (its documented bound)                     2^-22
-    1 + e, quotient, product with the up value: three roundings                           3 * 2^-24
+    exponential e = exp(-gate): 2 + 1.173 |gate| units of 2^-23 (the documented bound of the quick one), of which
+    the part e / (1 + e) = sigmoid(-gate) reaches 1 + e                                   (2 + 1.173 |gate|) sigmoid(-gate) 2^-23
+    quotient: 2 units of 2^-23 (documented)                                               2^-22
+    1 + e, product with the up value: two roundings                                       2 * 2^-24
     value + remainder: a rounding of a rounding, (eps / 2)^2                              2^-22 (fp16), 2^-16 (bf16)
     their sum in the tensor core: two units of 2^-23                                      2^-22
-    together, relative to the gated value                                                 < 2^-20 (+ 2^-16 for bf16)
+    all but the exponential, relative to the gated value                                  3.5 * 2^-22, or 2.5 * 2^-22 + 2^-16
 
 and, where the pair is scaled to its slot's largest value (to 2^14 at least), half of fp16's smallest step 2^-24: 2^-39 of that
 largest value. The result is then rounded once."""
@@ -47,11 +49,11 @@ def test_moe_gated_values_far_beyond_the_range_of_fp16(pkg, cuda, tokens):
 
 # what the gates are (x's first coordinate times a weight of about this size), the up value, the weight behind them
 REGIMES = {"ordinary": (1.0, 1.0, 2.0 ** 6, 1.0), "small": (2.0 ** -8, 2.0 ** -3, 2.0 ** -8, 2.0 ** 13), "smallest": (2.0 ** -6, 2.0 ** -4, 2.0 ** -12, 2.0 ** 15),
-           "large": (2.0 ** 7, 2.0 ** 7, 2.0 ** 16, 2.0 ** -20)}
+           "large": (2.0 ** 7, 2.0 ** 7, 2.0 ** 16, 2.0 ** -20), "closed": (1.0, -36.0, 2.0 ** 36, 2.0 ** 15)}
 
 
 def one_number_each(torch, name, tokens, regime, seed):
-    """x, logits, w13, w2, and in 64 bits: Y, per (token, hidden) the size of the token's largest gated value times the weight."""
+    """x, logits, w13, w2, and in 64 bits: Y, the size of a token's largest gated value times the weight, the gates."""
     experts, width = 3, 72
     g = torch.Generator(device="cuda").manual_seed(seed)
     t = dt(torch, name)
@@ -69,7 +71,7 @@ def one_number_each(torch, name, tokens, regime, seed):
     e = logits.argmax(dim=1)
     gate = x[:, :1].double() * w13[e, :width, 0].double()
     h = gate * torch.sigmoid(gate) * up
-    return x, logits, w13, w2, h * back, h.abs().amax(dim=1, keepdim=True) * back
+    return x, logits, w13, w2, h * back, h.abs().amax(dim=1, keepdim=True) * back, gate
 
 
 @pytest.mark.gpu
@@ -77,7 +79,7 @@ def one_number_each(torch, name, tokens, regime, seed):
 @pytest.mark.parametrize("regime", REGIMES)
 @pytest.mark.parametrize("tokens", [1, 40, 64, 256])
 def test_moe_one_number_each(pkg, cuda, tokens, regime, name):
-    x, logits, w13, w2, want, largest = one_number_each(cuda, name, tokens, regime, tokens)
+    x, logits, w13, w2, want, largest, gate = one_number_each(cuda, name, tokens, regime, tokens)
     got = run_moe(pkg, cuda, x, logits, w13, w2, 1, True)[0]
-    rel = 2.0 ** -20 + (2.0 ** -16 if name == "bf16" else 0.0)
+    rel = (3.5 * 2.0 ** -22 if name == "fp16" else 2.5 * 2.0 ** -22 + 2.0 ** -16) + (2 + 1.173 * gate.abs()) * cuda.sigmoid(-gate) * 2.0 ** -23
     check_close(got, want, rel * want.abs() + 2.0 ** -39 * largest, name)
