@@ -16,7 +16,7 @@ and, where the pair is scaled to its slot's largest value (to 2^14 at least), ha
 largest value. The result is then rounded once."""
 import pytest
 
-from test_routed import check_close, check_moe, dt, moe_inputs, run_moe
+from test_routed import check_close, check_moe, dt, moe_inputs, moe_want, route_want, run_moe
 
 SIZES = [(1, 264, 72, 6, 2), (24, 264, 136, 5, 3), (64, 328, 1032, 4, 2), (150, 264, 72, 6, 2), (256, 136, 4168, 3, 1)]   # tokens, hidden, inner, experts, top_k
 
@@ -83,3 +83,124 @@ def test_moe_one_number_each(pkg, cuda, tokens, regime, name):
     got = run_moe(pkg, cuda, x, logits, w13, w2, 1, True)[0]
     rel = (3.5 * 2.0 ** -22 if name == "fp16" else 2.5 * 2.0 ** -22 + 2.0 ** -16) + (2 + 1.173 * gate.abs()) * cuda.sigmoid(-gate) * 2.0 ** -23
     check_close(got, want, rel * want.abs() + 2.0 ** -39 * largest, name)
+
+
+# ------------------------------------------------------------------------------------------------ the kernels that fp16 takes
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [3, 130])
+@pytest.mark.parametrize("inner", [8200, 20008])
+def test_moe_many_inner_rows(pkg, cuda, tokens, inner):
+    """More gated values of a slot than its cluster of blocks keeps in registers (16384), small ones among them."""
+    x, logits, w13, w2 = moe_inputs(cuda, "fp16", tokens, 72, inner, 3, inner)
+    check_moe(pkg, cuda, "fp16", x * 3e-3, logits, w13, w2 * 10.0, 2, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 9, 70])
+def test_moe_fp16_reads_nothing_of_experts_and_tokens_that_are_not_a_tokens_own(pkg, cuda, tokens):
+    """Nor does a slot's scale follow another's values, or values that are not finite."""
+    torch = cuda
+    x, logits, w13, w2 = moe_inputs(torch, "fp16", tokens, 328, 72, 10, 9)
+    logits[:, [0, 4, 9]] = -float("inf")
+    clean = [t.clone() for t in run_moe(pkg, torch, x, logits, w13, w2, 3, True)]
+    for e in (0, 4, 9):
+        w13[e], w2[e] = float("nan"), float("inf")
+    for got, want in zip(run_moe(pkg, torch, x, logits, w13, w2, 3, True), clean):
+        assert torch.equal(got, want)
+    x[0] *= 1000.0
+    others = run_moe(pkg, torch, x, logits, w13, w2, 3, True)[0]
+    assert torch.equal(others[1:], clean[0][1:])
+    x[0, 3] = float("nan")
+    y = run_moe(pkg, torch, x, logits, w13, w2, 3, True)[0]
+    assert y[0].isnan().all() and torch.equal(y[1:], clean[0][1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [2, 30, 200])
+def test_moe_an_infinite_gated_value_beside_finite_ones(pkg, cuda, tokens):
+    """An infinity of UP gives infinities of its weights' signs, whatever the finite values beside it are."""
+    torch = cuda
+    x, logits, w13, w2 = moe_inputs(torch, "fp16", tokens, 72, 72, 2, 5)
+    x[:, 0] = 60000.0
+    w13[:, :, 0] = 0
+    w13[:, 5, 0], w13[:, 72 + 5, 0] = 60000.0, float("inf")       # gate 3.6e9, up infinite
+    w13[:, 6, 0], w13[:, 72 + 6, 0] = 60000.0, 60000.0            # a finite gated value of 1.3e19
+    w2[w2 == 0] = 1.0
+    y = run_moe(pkg, torch, x, logits, w13, w2, 1, True)[0]
+    e = logits.argmax(dim=1)
+    assert y.isinf().all() and torch.equal(y > 0, w2[e, :, 5] > 0)
+
+
+@pytest.mark.gpu
+def test_moe_fp16_chains_without_pauses_keep_their_order(pkg, cuda):
+    torch = cuda
+    for tokens in (1, 20, 100):
+        x, _, w13, w2 = moe_inputs(torch, "fp16", tokens, 256, 64, 8, 3)
+        logits = torch.randn(tokens, 8, device="cuda")
+        workspace = torch.empty(pkg.moe_workspace_bytes(tokens, 256, 64, 8, 2), dtype=torch.uint8, device="cuda")
+
+        def run(pause):
+            v = x
+            for _ in range(40):
+                d = pkg.moe(v, logits, w13, w2, 2, workspace=workspace)[0]
+                d = pkg.moe(d, logits, w13, w2 * 30.0, 2, workspace=workspace)[0].float()
+                v = (d * d.square().mean(dim=1, keepdim=True).rsqrt()).half()      # the gate makes a step quadratic: each row is kept at one size
+                if pause:
+                    torch.cuda.synchronize()
+            return v
+
+        slow = run(True)
+        assert bool(slow.isfinite().all()) and torch.equal(run(False), slow) and pkg.device_status()[0] == pkg.OK
+
+
+@pytest.mark.gpu
+def test_moe_fp16_graphs_replayed_side_by_side(pkg, cuda):
+    """Captured calls of the two ways, on two streams, with new inputs of other sizes each time."""
+    torch = cuda
+    states = []
+    for tokens in (6, 70):
+        x, logits, w13, w2 = moe_inputs(torch, "fp16", tokens, 520, 4168, 5, tokens)
+        states.append(dict(x=x, logits=logits, w13=w13, w2=w2))
+    graphs, streams = [], [torch.cuda.Stream() for _ in states]
+    for s in states:
+        pkg.moe(s["x"], s["logits"], s["w13"], s["w2"], 3)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s["out"] = pkg.moe(s["x"], s["logits"], s["w13"], s["w2"], 3)
+        graphs.append(g)
+    for seed, size in enumerate((1.0, 1e-2, 30.0)):
+        for s in states:
+            x, logits, _, _ = moe_inputs(torch, "fp16", s["x"].shape[0], 520, 8, 5, seed)
+            s["x"].copy_(x * size), s["logits"].copy_(logits)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert pkg.device_status()[0] == pkg.OK
+        for s in states:
+            y, ids, weights = s["out"]
+            want_ids, want_weights = route_want(torch, s["logits"], 3, True)
+            assert torch.equal(ids, want_ids)
+            check_close(y, *moe_want(torch, s["x"], s["w13"], s["w2"], want_ids, want_weights), "fp16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [2, 200])
+def test_moe_fp16_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(pkg, cuda, tokens):
+    torch = cuda
+    x, logits, w13, w2 = moe_inputs(torch, "fp16", tokens, 16384, 16384, 2, 5)
+    call = lambda: pkg.moe(x, logits, w13, w2, 1)[0]
+    want = call()
+    assert pkg.device_status()[0] == pkg.OK
+    pkg.set_wait_budget_ns(1)
+    try:
+        call()
+        status, info = pkg.device_status()
+    finally:
+        pkg.set_wait_budget_ns(2_000_000_000)
+    assert status == pkg.DEVICE_TIMEOUT and 1000 <= info[2] < 1500, (status, info)
+    assert torch.equal(call(), want) and pkg.device_status()[0] == pkg.OK
