@@ -302,7 +302,8 @@ def gemm_lora(A, Bt, lora_a, lora_b, row_adapter, lora_scale=None, D=None, works
     A (m, k), Bt (n, k), lora_a (adapters, rank, k), lora_b (adapters, n, rank) and D (m, n): contiguous torch CUDA tensors of
     one 16-bit type; row_adapter (m,) int32, an entry outside [0, adapters) = no adapter; lora_scale (adapters,) fp32 or None.
     D and the workspace are allocated, on the stream of the call, when not given. stream: a cudaStream_t as an int (None =
-    torch's current one); the operands must be ready there. Raises ValueError for tensors that do not fit together and
+    torch's current one); the operands must be ready there, and stay alive until that stream has read them, which torch's
+    allocator does not know of (Tensor.record_stream tells it). Raises ValueError for tensors that do not fit together and
     B200Error for what the library refuses."""
     torch = _torch()
     if A.dim() != 2 or Bt.dim() != 2 or lora_a.dim() != 3:

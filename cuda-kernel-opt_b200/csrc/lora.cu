@@ -9,24 +9,25 @@
 //
 // Why not on the tensor core, as further columns of K: the zero that stands for "not this row's adapter" does not mask an infinity
 // or a NaN among an adapter's weights, so a request would see other requests' adapters; and a decode step in which every
-// row has another adapter would feed it one useful row at a time. Only where 32 rows in a row have one adapter, as in a
+// row has another adapter would feed it one useful row at a time. (Columns of tensor memory of their own per adapter, of which
+// only its rows are kept, as the first product does it, would need no zeros; there are none left beside two accumulators.) Only where 32 rows in a row have one adapter, as in a
 // prompt, does the tensor core take them (u then as a pair of 16-bit numbers, value and remainder), as long as u fits those.
 //
-// Three forms, by the numbers of rows and columns:
+// Three forms, by the numbers of rows and columns (times: on the device, in a graph, SM clock 1965 MHz if nothing else is said):
 //   up to 256     one CTA per tile of 128 columns, all rows. Reading B bounds it: 16 x 28672 x 8192, rank 16, takes 77 us, 6.3 TB/s; 128
-//                 rows, rank 32, any of 64 adapters per row, 126 us, 4.8 TB/s. The K blocks of all tiles are cut into one equal
+//                 rows, rank 32, any of 64 adapters per row, 128 to 138 us, 4.4 to 4.8 TB/s. The K blocks of all tiles are cut into one equal
 //                 stretch per CTA (Cut), so that every SM streams all the time; a tile that spans several leaves parts in the
 //                 workspace, and the last of its CTAs to finish adds them in ascending order. No CTA waits for another,
 //                 nothing is added atomically. (A CTA pair per 256 columns, which halves what the rows of A cost between L2 and
 //                 SMs, measured the same within 1 % from 65 to 256 rows.)
 //   few columns   the same with the rows in several blocks, each with its own stretches: more CTAs share the work, the rows' adapters
 //                 above all. 225 x 672 x 3120, rank 72, any of 14 adapters per row: 107 -> 48 us, 25 x 384 x 744, rank 120: 39 ->
-//                 19.5; beyond 256 rows while waves would have at most 18 tiles: 535 x 312 x 360, rank 72, 43 prompts: 134 ->
-//                 39 us against waves, 1024 x 2048 x 2048 (32 tiles): 30 in waves, 45 in blocks. A kernel of its own, the
+//                 18.6; beyond 256 rows while waves would have at most 18 tiles: 535 x 312 x 360, rank 72, 43 prompts: 134 ->
+//                 39 us against waves, 1024 x 2048 x 2048 (32 tiles): 33 in waves, 45 in blocks. A kernel of its own, the
 //                 general walk costs the form above 5 % of its smallest calls.
 //   more          a CTA pair per 256 x 256 tile, whole tiles in waves, the tensor core bounds it: 4096 x 8192 x 8192, rank 64, eight
-//                 prompts, takes 400 us, 1.40 PFLOP/s, the rate that the power limit leaves a plain product. 512 rows of eight
-//                 prompts take 78 us, two calls of 256 rows 125.
+//                 prompts, takes 450 us call after call at the 1365 MHz that the power limit leaves, 1.25 PFLOP/s; the best of
+//                 short runs 385 us. 512 rows of eight prompts take 78 us, two calls of 256 rows 120.
 //
 // u comes first, from lora_shrink_dot_kernel (few rows) or lora_list_kernel, lora_shrink_kernel and lora_join_kernel. They let the product
 // start before they are done; only its warps that need u wait.

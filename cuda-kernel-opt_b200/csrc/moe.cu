@@ -19,9 +19,9 @@
 //                                 cost as much accuracy as the rounding of the result); the last CTA of a tile of Y adds
 //                                 its parts and the weighted choices. With fp16 the pairs have to be scaled, for which a
 //                                 slot's largest value has to be known: moe_gate_kernel makes them in between, at the price of
-//                                 a kernel in the chain (2 tokens, 8 experts of 1024 x 512, top 2: 15.6 us with bf16, 20.0 with
-//                                 fp16; one token, 8 of 128 experts of 2048 x 768: 28.5 and 33; 16 tokens, 64 experts of 4096 x
-//                                 2048, top 6: 398 and 405)
+//                                 a kernel in the chain (2 tokens, 8 experts of 1024 x 512, top 2: 15.5 us with bf16, 20.0 with
+//                                 fp16; one token, 8 of 128 experts of 2048 x 768: 28.6 and 33.1; 16 tokens, 64 experts of 4096 x
+//                                 2048, top 6: 398 and 406)
 // beyond that five, because each CTA would spend too long on the choice, the gated values and the last sums (48 tokens, 32 experts
 // of 1024 x 512, top 4: 38 against 41 us; 256 tokens, 128 experts of 2048 x 768, top 8: 230 against 404):
 //   moe_route_kernel              a cluster of up to eight blocks: the choice per token (one warp each), the chosen experts' tokens
@@ -31,10 +31,10 @@
 //   moe_combine_kernel            parts and weighted choices of a token, one rounding
 //
 // All are launched as programmatic dependents: DOWN_FEW starts as soon as UP_FEW runs (two CTAs fit an SM), fills its ring with weights and
-// waits only before it reads UP's sums. Measured as device time in a graph: 16 tokens, 64 experts of 4096 x 2048, top 6, 397 us:
-// 6.4 TB/s, 98 % of the copy rate; 64 tokens, experts of 4096 x 1408, 350 us, 96 %; 256 tokens as above 228 us, 81 %: the
-// activations and sums of 2048 slots cross the L2 beside the weights; one token, 8 of 128 experts of 2048 x 768, 28 us, 40 %:
-// the choice, two starts and two joins of some microseconds each frame 11 us of reading.
+// waits only before it reads UP's sums. Measured as device time in a graph, bf16: 16 tokens, 64 experts of 4096 x 2048, top 6, 398 us:
+// 6.4 TB/s, 98 % of the copy rate; 64 tokens, experts of 4096 x 1408, 354 us, 95 %; 256 tokens as above 229 us, 80 %: the
+// activations and sums of 2048 slots cross the L2 beside the weights; one token, 8 of 128 experts of 2048 x 768, 28.6 us, 40 %:
+// the choice, two starts and two joins frame 11 us of reading.
 #include <cuda_runtime.h>
 
 #include <cfloat>

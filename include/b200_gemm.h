@@ -288,7 +288,11 @@ int b200_session_gemm_host_sharded(b200_session *s, int dtype, const void *hA_ro
 
 /* Products whose rows choose their own weights (decode and prompt steps of a language model). They have no
  * counterpart in the reference, whose launchers multiply every row of A with the same B. Operands and
- * outputs are fp16 or bf16 (dtype), sums are fp32, outputs are rounded once. As everywhere here the calls
+ * outputs are fp16 or bf16 (dtype), sums are fp32, outputs are rounded once. Two intermediate values are multiplied
+ * again as pairs of 16-bit numbers: the gated values of b200_moe, which then err by 2^-16 of themselves with bf16 and with fp16 by 2^-22
+ * of themselves and 2^-39 of the token's largest one in that expert; and, beyond 256 rows, A * lora_a^T where 32 rows
+ * share an adapter, which errs by 2^-16 of itself with bf16 and with fp16 by 2^-22 of itself or 2^-17 of the largest of its
+ * eight neighbouring ranks (where that is below 2^-8, fp32 is used). As everywhere here the calls
  * allocate nothing, enqueue on the given stream and return; the same inputs give the same bits. The workspace
  * (256-byte aligned, any contents) holds intermediate sums: calls that may overlap on the GPU (two streams,
  * two graphs replayed side by side) need one each. Its size is asked for with the sizes of the call: fewer rows or
